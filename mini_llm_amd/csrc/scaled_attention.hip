@@ -1,0 +1,329 @@
+// Attention over a cache of 8 bits (scaled_blocks.h, scaled_sweep.h).
+//
+// A token at position p attends to the keys max(0, p - window + 1) .. p of its request (window 0: all; with kept first keys also to those;
+// or, with chunks, to the keys of its own chunk up to p). A row without a request, or at a position before the first, sees nothing:
+// zeros.
+#include "scaled_sweep.h"
+
+namespace {
+
+struct AttendArguments {
+    const void* q;
+    long long q_stride;
+    void* out;
+    long long out_stride;
+    const int* token_request;
+    const int* positions;
+    const int* q_starts;
+    const int* context_lens;
+    const int* block_tables;
+    const float* sinks;
+    ScaledPlanes planes;
+    int max_blocks, n_tables, n_rows, n_heads, window, chunk, keep, aligned, negative, wide_out, out_packed;
+    ScoreScale scale;
+    float sink_factor;   // log2 e where weights are powers of two
+};
+
+// One result: of row `row`, element `at` of its n_heads * head_size.
+template <typename T>
+__device__ __forceinline__ void put_result(const AttendArguments& a, int row, int at, float value) {
+    const size_t index = a.out_packed ? packed_element<T>(row, at, a.n_heads * a.planes.head_size) : (size_t)row * a.out_stride + at;
+    if (sizeof(T) == 4 || !a.wide_out) static_cast<T*>(a.out)[index] = from_float<T>(value);
+    else static_cast<float*>(a.out)[index] = value;
+}
+
+// What a row sees, or no tile at all.
+struct RowView {
+    int request, position, first;
+    __device__ __forceinline__ RowView(const AttendArguments& a, int row) {
+        request = a.token_request[row];
+        position = a.positions[row];
+        if (request >= a.n_tables) request = -1;
+        position = min(position, (int)min((long long)a.max_blocks << a.planes.page_shift, 2147483647LL) - 1);
+        first = scaled_first_key(max(position, 0), a.window, a.chunk);
+    }
+    __device__ __forceinline__ bool sees() const { return request >= 0 && position >= 0; }
+};
+
+// Rows by themselves (decoding, short portions, and whatever else comes without the shape of portions): a block per row, group of up to 16
+// heads that share a key/value head, and run of `run_tiles` tiles; its waves take the run's tiles in turn and meet in LDS. Rows of more
+// than one run leave unnormalised sums, maximum and weight per run in `parts` ([row, head, run, head_size + 2]) for the kernel below.
+// What bounds it is the cache's bytes: 2 (head_size + 0.25) a key for all heads of the group together.
+template <typename T, int HD>
+__global__ __launch_bounds__(HD == 64 ? 1024 : HD == 128 ? 512 : 256) void scaled_rows_attention_kernel(AttendArguments a, int run_tiles, int n_runs, float* __restrict__ parts) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    typedef ScaledSweep<HD, 1, WIDE> Sweep;
+    extern __shared__ float meeting[];   // [wave][column][head_size + 4]
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, waves = blockDim.x / WAVE;
+    const int row = blockIdx.x, run = blockIdx.z;
+    const int head_size = a.planes.head_size, group = a.n_heads / a.planes.n_kv_heads, sets = ceil_div(group, 16);
+    const int kv_head = blockIdx.y / sets, head0 = kv_head * group + (blockIdx.y % sets) * 16;
+    const int columns = min(16, (kv_head + 1) * group - head0);
+    const RowView view(a, row);
+    if (!view.sees()) {
+        if (run == 0)
+            for (int i = threadIdx.x; i < columns * head_size; i += blockDim.x) put_result<T>(a, row, head0 * head_size + i, 0.0f);
+        return;
+    }
+    const TileRange range(view.first, view.position, a.keep);
+    const int begin = run * run_tiles, end = run == n_runs - 1 ? range.count : min(range.count, begin + run_tiles);
+    if (begin >= end) return;
+    const bool alone = n_runs == 1 || range.count <= run_tiles;
+
+    Sweep sweep;
+    sweep.init();
+    const int column = lane % 16;
+    sweep.template load_query<T>(0, column < columns ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride + (head0 + column) * head_size : nullptr, head_size, a.aligned, a.negative, lane);
+    const int first[1] = {view.first}, last[1] = {view.position};
+    sweep.tiles(range, begin + wave, waves, end, a.block_tables + (size_t)view.request * a.max_blocks, a.planes, kv_head, a.scale, first, last, view.first, view.position, a.keep, lane);
+
+    const int pitch = head_size + 4;
+    float l = sweep.l[0];
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+    // the maximum is the same in the four lanes of a column: it is only raised together
+    float* const mine = meeting + (wave * columns + column) * pitch;
+    if (column < columns) {
+#pragma unroll
+        for (int dt = 0; dt < Sweep::DT; dt++)
+            if (dt * 16 < head_size) *reinterpret_cast<f32x4*>(mine + dt * 16 + 4 * (lane / 16)) = sweep.o[0][dt];
+        if (lane < 16) {
+            mine[head_size] = sweep.m[0];
+            mine[head_size + 1] = l;
+        }
+    }
+    __syncthreads();
+    // a wave without tiles has m = NO_SCORE, l = 0 and sums of 0
+    for (int i = threadIdx.x; i < columns * head_size; i += blockDim.x) {
+        const int c = i / head_size, d = i % head_size;
+        const float* const at = meeting + c * pitch;
+        float top = NO_SCORE;
+        for (int w = 0; w < waves; w++) top = fmaxf(top, at[w * columns * pitch + head_size]);
+        float total = 0.0f, value = 0.0f;
+        for (int w = 0; w < waves; w++) {
+            const float factor = weight_of<WIDE>(at[w * columns * pitch + head_size] - top);
+            total += at[w * columns * pitch + head_size + 1] * factor;
+            value += at[w * columns * pitch + d] * factor;
+        }
+        if (alone) {
+            if (a.sinks) total += weight_of<WIDE>(a.sinks[head0 + c] * a.sink_factor - top);
+            put_result<T>(a, row, (head0 + c) * head_size + d, value / total);
+        } else {
+            float* const part = parts + (((size_t)row * a.n_heads + head0 + c) * n_runs + run) * (head_size + 2);
+            part[d] = value;
+            if (d == 0) {
+                part[head_size] = top;
+                part[head_size + 1] = total;
+            }
+        }
+    }
+}
+
+// Puts the runs of a row's head together: a block a (row, head).
+template <typename T>
+__global__ __launch_bounds__(64) void scaled_merge_kernel(AttendArguments a, int run_tiles, int n_runs, const float* __restrict__ parts) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, head_size = a.planes.head_size;
+    const RowView view(a, row);
+    if (!view.sees()) return;
+    const TileRange range(view.first, view.position, a.keep);
+    if (range.count <= run_tiles) return;
+    const int runs = min(ceil_div(range.count, run_tiles), n_runs);
+    const float* const mine = parts + ((size_t)row * a.n_heads + head) * n_runs * (head_size + 2);
+    const int pitch = head_size + 2;
+    float top = NO_SCORE;
+    for (int r = lane; r < runs; r += WAVE) top = fmaxf(top, mine[r * pitch + head_size]);
+    top = wave_max_total(top);
+    float total = 0.0f;
+    for (int r = lane; r < runs; r += WAVE) total += mine[r * pitch + head_size + 1] * weight_of<WIDE>(mine[r * pitch + head_size] - top);
+    total = wave_total(total);
+    if (a.sinks) total += weight_of<WIDE>(a.sinks[head] * a.sink_factor - top);
+    for (int d = lane; d < head_size; d += WAVE) {
+        float value = 0.0f;
+        for (int r = 0; r < runs; r++) value += mine[r * pitch + d] * weight_of<WIDE>(mine[r * pitch + head_size] - top);
+        put_result<T>(a, row, head * head_size + d, value / total);
+    }
+}
+
+// Portions of prompts: a block per (request, head, tile of 16 CT rows), whose waves hold all those rows and take the tiles of keys in turn,
+// each with statistics of its own, and meet in LDS. Tiles with the most keys come first.
+template <typename T, int HD, int CT>
+__global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void scaled_tiles_attention_kernel(AttendArguments a) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    typedef ScaledSweep<HD, CT, WIDE> Sweep;
+    constexpr int ROWS = 16 * CT, WAVES = 4;
+    __shared__ float meeting[WAVES / 2][CT][Sweep::DT + 1][4][WAVE];   // what half of the waves hold, lane by lane
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const int request = blockIdx.z, head = blockIdx.y, head_size = a.planes.head_size;
+    const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
+    const int row0 = (gridDim.x - 1 - blockIdx.x) * ROWS;
+    const int context = a.context_lens[request];
+    if (row0 >= q_len || context < 0 || q_first < 0) return;   // (a negative context: a padding request, whose rows are nobody's)
+    const int kv_head = head / (a.n_heads / a.planes.n_kv_heads);
+    const int reach = (int)min((long long)a.max_blocks << a.planes.page_shift, 2147483647LL) - 1;
+    const int position0 = min(context + row0, reach), position1 = min(context + min(row0 + ROWS, q_len) - 1, reach);
+
+    Sweep sweep;
+    sweep.init();
+    int first[CT], last[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int local = row0 + 16 * ct + lane % 16;
+        const bool valid = local < q_len;
+        last[ct] = min(context + (valid ? local : q_len - 1), reach);
+        first[ct] = scaled_first_key(last[ct], a.window, a.chunk);
+        sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
+    }
+    const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
+    sweep.tiles(range, wave, WAVES, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale, first, last,
+                scaled_first_key(position1, a.window, a.chunk), position0, a.keep, lane);
+
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        sweep.l[ct] += __shfl_xor(sweep.l[ct], 16, WAVE);
+        sweep.l[ct] += __shfl_xor(sweep.l[ct], 32, WAVE);
+    }
+    // the waves' sums: the upper half's into the lower half's, then wave 1's into wave 0's
+#pragma unroll
+    for (int half = WAVES / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (wave >= half && wave < 2 * half) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+#pragma unroll
+                for (int dt = 0; dt < Sweep::DT; dt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) meeting[wave - half][ct][dt][i][lane] = sweep.o[ct][dt][i];
+                meeting[wave - half][ct][Sweep::DT][0][lane] = sweep.m[ct];
+                meeting[wave - half][ct][Sweep::DT][1][lane] = sweep.l[ct];
+            }
+        }
+        __syncthreads();
+        if (wave < half) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const float other = meeting[wave][ct][Sweep::DT][0][lane], top = fmaxf(sweep.m[ct], other);
+                const float mine = weight_of<WIDE>(sweep.m[ct] - top), theirs = weight_of<WIDE>(other - top);
+                sweep.m[ct] = top;
+                sweep.l[ct] = sweep.l[ct] * mine + meeting[wave][ct][Sweep::DT][1][lane] * theirs;
+#pragma unroll
+                for (int dt = 0; dt < Sweep::DT; dt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sweep.o[ct][dt][i] = sweep.o[ct][dt][i] * mine + meeting[wave][ct][dt][i][lane] * theirs;
+            }
+        }
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int local = row0 + 16 * ct + lane % 16;
+        if (local >= q_len) continue;
+        float total = sweep.l[ct];
+        if (a.sinks) total += weight_of<WIDE>(a.sinks[head] * a.sink_factor - sweep.m[ct]);
+        const float inverse = 1.0f / total;
+#pragma unroll
+        for (int dt = 0; dt < Sweep::DT; dt++)
+            if (dt * 16 < head_size)
+#pragma unroll
+                for (int i = 0; i < 4; i++) put_result<T>(a, q_first + local, head * head_size + dt * 16 + 4 * (lane / 16) + i, sweep.o[ct][dt][i] * inverse);
+    }
+}
+
+int refuse_attend(const char* what, const AttendArguments& a, int page_size, int dtype) {
+    const ScaledPlanes& p = a.planes;
+    MLLM_REQUIRE(a.n_rows >= 0 && a.n_heads > 0 && p.n_kv_heads > 0 && a.max_blocks > 0 && a.n_tables > 0 && p.num_pages > 0, "%s: bad sizes", what);
+    MLLM_REQUIRE(a.n_heads % p.n_kv_heads == 0, "%s: %d heads do not divide into %d key/value heads", what, a.n_heads, p.n_kv_heads);
+    MLLM_REQUIRE(p.head_size > 0 && p.head_size % 16 == 0 && p.head_size <= SCALED_MAX_HEAD, "%s: heads of %d (a multiple of 16 up to %d)", what, p.head_size, SCALED_MAX_HEAD);
+    MLLM_REQUIRE(page_size >= BLOCK_TOKENS && (page_size & (page_size - 1)) == 0, "%s: page size %d is no power of two of at least %d", what, page_size, BLOCK_TOKENS);
+    MLLM_REQUIRE(dtype == MLLM_F32 || dtype == MLLM_BF16, "%s: unknown dtype %d", what, dtype);
+    MLLM_REQUIRE(a.window >= 0 && a.chunk >= 0 && !(a.window && a.chunk), "%s: bad window or chunk", what);
+    MLLM_REQUIRE(a.keep >= 0 && (a.keep == 0 || a.window > 0), "%s: first keys are kept beside a window", what);
+    MLLM_REQUIRE(a.q_stride >= (long long)a.n_heads * p.head_size && a.out_stride >= (long long)a.n_heads * p.head_size, "%s: rows are too short for the heads", what);
+    MLLM_REQUIRE(!(a.wide_out && a.out_packed), "%s: rows in the packed layout leave in the queries' type", what);
+    return 0;
+}
+
+AttendArguments attend_arguments(const void* q, long long q_stride, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales, void* out,
+                                 long long out_stride, const int* block_tables, int max_blocks, int n_tables, int num_pages, int n_rows, int n_heads, int n_kv_heads,
+                                 int head_size, int page_size, int window, float scale, int dtype, float softcap, const float* sinks, int chunk, int keep, int wide_out) {
+    int shift = 0;
+    while ((1 << shift) < page_size) shift++;
+    const float unit = dtype == MLLM_F32 ? 1.0f : 1.4426950408889634f, size = scale < 0.0f ? -scale : scale;
+    AttendArguments a = {};
+    a.q = q, a.q_stride = q_stride, a.out = out, a.out_stride = out_stride, a.block_tables = block_tables, a.sinks = sinks;
+    a.planes = {(const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales, num_pages, n_kv_heads, head_size, shift};
+    a.max_blocks = max_blocks, a.n_tables = n_tables, a.n_rows = n_rows, a.n_heads = n_heads, a.window = window, a.chunk = chunk, a.keep = keep;
+    a.aligned = (uintptr_t)q % 16 == 0 && q_stride * (dtype == MLLM_F32 ? 4 : 2) % 16 == 0;
+    a.negative = scale < 0.0f, a.wide_out = wide_out;
+    // (a factor of zero would make numbers that are none of masked scores: 1e-30 leaves as little between any two others)
+    a.scale = {size * unit > 1e-30f ? size * unit : 1e-30f, softcap > 0.0f ? size / softcap : 0.0f, softcap > 0.0f ? softcap * unit : 0.0f};
+    a.sink_factor = unit;
+    return a;
+}
+
+}  // namespace
+
+// Rows by themselves. The keys of a row are cut into runs of run_tiles tiles of 64, n_runs of them at most: a shorter sequence has fewer, and
+// the last run of a longer one takes all that is left; n_runs > 1 needs `parts`, n_rows * n_heads * n_runs * (head_size + 2) floats.
+MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales, void* out,
+                                        long long out_stride, const int* token_request, const int* positions, const int* block_tables, int max_blocks, int n_tables,
+                                        int num_pages, int n_rows, int n_heads, int n_kv_heads, int head_size, int page_size, int window, float scale, int dtype,
+                                        float softcap, const float* sinks, int chunk, int keep, int wide_out, int out_packed, int waves, int run_tiles, int n_runs, float* parts,
+                                        hipStream_t stream) {
+    AttendArguments a = attend_arguments(q, q_stride, k_codes, k_scales, v_codes, v_scales, out, out_stride, block_tables, max_blocks, n_tables, num_pages, n_rows, n_heads,
+                                         n_kv_heads, head_size, page_size, window, scale, dtype, softcap, sinks, chunk, keep, wide_out);
+    a.token_request = token_request, a.positions = positions, a.out_packed = out_packed;
+    if (int status = refuse_attend("scaled_attention_rows", a, page_size, dtype)) return status;
+    const int padded = head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256, most = 1024 / padded;
+    MLLM_REQUIRE(waves >= 1 && waves <= most && run_tiles >= 1 && n_runs >= 1 && n_runs <= 65535 && (n_runs == 1 || parts != nullptr),
+                 "scaled_attention_rows: %d waves (1..%d), runs of %d tiles, %d runs (with memory for more than one)", waves, most, run_tiles, n_runs);
+    const int group = n_heads / n_kv_heads, columns = group < 16 ? group : 16;
+    const size_t lds = (size_t)waves * columns * (head_size + 4) * sizeof(float);
+    MLLM_REQUIRE(lds <= 65536, "scaled_attention_rows: %d waves of %d heads need more LDS than a block has", waves, columns);
+    if (n_rows == 0) return 0;
+    const dim3 grid(n_rows, n_kv_heads * ceil_div(group, 16), n_runs);
+    MLLM_REQUIRE(grid.y <= 65535, "scaled_attention_rows: too many heads for one launch");
+    mllm_count_kernel(MLLM_K_SCALED_ATTENTION_ROWS);
+#define ROWS_CASE(T)                                                                                                       \
+    if (padded == 64) scaled_rows_attention_kernel<T, 64><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);         \
+    else if (padded == 128) scaled_rows_attention_kernel<T, 128><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);  \
+    else scaled_rows_attention_kernel<T, 256><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);
+    if (dtype == MLLM_F32) {
+        ROWS_CASE(float)
+    } else {
+        ROWS_CASE(bf16_t)
+    }
+#undef ROWS_CASE
+    if (int status = mllm_check_launch("scaled_attention_rows")) return status;
+    if (n_runs == 1) return 0;
+    mllm_count_kernel(MLLM_K_SCALED_ATTENTION_MERGE);
+    if (dtype == MLLM_F32) scaled_merge_kernel<float><<<dim3(n_rows, n_heads), WAVE, 0, stream>>>(a, run_tiles, n_runs, parts);
+    else scaled_merge_kernel<bf16_t><<<dim3(n_rows, n_heads), WAVE, 0, stream>>>(a, run_tiles, n_runs, parts);
+    return mllm_check_launch("scaled_attention_merge");
+}
+
+// Portions: the rows of request r are q_starts[r] .. q_starts[r + 1] - 1, the first of them at position context_lens[r] (negative: nobody's rows).
+MLLM_API int mllm_scaled_attention_tiles(const void* q, long long q_stride, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales, void* out,
+                                         long long out_stride, const int* q_starts, const int* context_lens, const int* block_tables, int max_blocks, int n_requests,
+                                         int num_pages, int n_rows, int max_q_len, int n_heads, int n_kv_heads, int head_size, int page_size, int window, float scale, int dtype,
+                                         float softcap, const float* sinks, int chunk, int keep, int wide_out, hipStream_t stream) {
+    AttendArguments a = attend_arguments(q, q_stride, k_codes, k_scales, v_codes, v_scales, out, out_stride, block_tables, max_blocks, n_requests, num_pages, n_rows, n_heads,
+                                         n_kv_heads, head_size, page_size, window, scale, dtype, softcap, sinks, chunk, keep, wide_out);
+    a.q_starts = q_starts, a.context_lens = context_lens;
+    if (int status = refuse_attend("scaled_attention_tiles", a, page_size, dtype)) return status;
+    MLLM_REQUIRE(n_requests <= 65535 && n_heads <= 65535, "scaled_attention_tiles: too many requests or heads for one launch");
+    if (n_rows == 0 || max_q_len <= 0) return 0;
+    mllm_count_kernel(MLLM_K_SCALED_ATTENTION_TILES);
+#define TILES_CASE(T, HD, CT) scaled_tiles_attention_kernel<T, HD, CT><<<dim3(ceil_div(max_q_len, 16 * CT), n_heads, n_requests), 256, 0, stream>>>(a)
+    if (dtype == MLLM_F32) {
+        if (head_size <= 64) TILES_CASE(float, 64, 2);
+        else if (head_size <= 128) TILES_CASE(float, 128, 2);
+        else TILES_CASE(float, 256, 1);
+    } else {
+        if (head_size <= 64) TILES_CASE(bf16_t, 64, 4);
+        else if (head_size <= 128) TILES_CASE(bf16_t, 128, 4);
+        else TILES_CASE(bf16_t, 256, 2);
+    }
+#undef TILES_CASE
+    return mllm_check_launch("scaled_attention_tiles");
+}

@@ -1,0 +1,324 @@
+// One wave's pass over tiles of 64 keys (four blocks) of a cache of 8 bits (scaled_blocks.h) for up to 16 CT columns: the queries that
+// share a key/value head and are looked at together (heads of a group that decode, or neighbouring rows of a prompt).
+//
+// S^T = K . Q^T and O^T = V^T . P^T on the 16 x 16 x 32 matrix instruction, scores and sums in 32-bit. With lane = 16 q + r:
+//  * Product t of a tile takes key 16 (r / 4) + 4 t + r % 4 as its row r, so that a lane's four scores of products 0 .. 3 are those of
+//    column r and all sixteen keys of block q: what it needs to be the operand of the second product (its quarter of the keys),
+//    with no exchange between lanes. (The order of the keys inside a product is free as long as both operands agree.)
+//  * A 16-byte load is 16 elements of one key (two quarters of a product's 32) or the 16 tokens of one value element: operands as they
+//    lie in the cache, but for their conversion to bfloat16, which is exact and multiplies by the block's scale on the way
+//    (v_cvt_scalef32_pk_bf16_fp8: two numbers an instruction).
+//  * The running maximum of a column is raised only in a tile with a score more than 8 above it (weights up to 2^8, or e^8, in between):
+//    most tiles have no exchange between lanes and no rescaling at all.
+// WIDE (32-bit queries and results): queries and weights go through the products as three bfloat16 pieces that add up to them exactly, so
+// every product of a query or weight with a held number is exact in 32-bit.
+#pragma once
+
+#include "scaled_blocks.h"
+
+constexpr int TILE_KEYS = 64;
+constexpr float NO_SCORE = -3.0e38f;       // the running maximum before any key: finite, so that nothing seen differs from it by no number
+constexpr float SCORE_SLACK = 8.0f;
+
+// The first key a query at `position` sees: the start of its chunk, or of its window, or key 0. It never falls as the position grows.
+__device__ __forceinline__ int scaled_first_key(int position, int window, int chunk) {
+    if (chunk > 0) return position - position % chunk;
+    return window > 0 ? max(0, position - window + 1) : 0;
+}
+
+struct ScaledPlanes {
+    const uint8_t* k_codes;
+    const float* k_scales;
+    const uint8_t* v_codes;
+    const float* v_scales;
+    int num_pages, n_kv_heads, head_size, page_shift;
+};
+
+// The keys that some query of a block sees, as tiles: those of the kept first keys, then from the first key's tile to the last's.
+struct TileRange {
+    int kept_tiles, first_tile, count;
+    int first_block, last_block, kept_blocks;   // blocks of 16 that are sure to be stored
+
+    __device__ __forceinline__ TileRange(int first_key, int last_key, int keep) {
+        keep = min(keep, first_key);
+        kept_blocks = (keep + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
+        kept_tiles = min((keep + TILE_KEYS - 1) / TILE_KEYS, first_key / TILE_KEYS);
+        first_tile = first_key / TILE_KEYS;
+        first_block = first_key / BLOCK_TOKENS;
+        last_block = last_key / BLOCK_TOKENS;
+        count = kept_tiles + last_key / TILE_KEYS - first_tile + 1;
+    }
+    __device__ __forceinline__ int first_key_of(int tile) const { return (tile < kept_tiles ? tile : first_tile + tile - kept_tiles) * TILE_KEYS; }
+    // a block that is sure to be stored in place of one that may not be (every key of such a one is masked)
+    __device__ __forceinline__ int stored(int block) const {
+        return block <= last_block && (block >= first_block || block < kept_blocks) ? block : last_block;
+    }
+};
+
+struct ScoreScale {
+    float factor;       // of a raw score: |scale|, times log2 e where weights are powers of two
+    float cap_in, cap;  // cap > 0: score <- cap tanh(raw cap_in), cap times log2 e where weights are powers of two
+};
+
+template <bool WIDE>
+__device__ __forceinline__ float weight_of(float x) {
+    if constexpr (WIDE) return expf(x);
+    else return __builtin_amdgcn_exp2f(x);
+}
+
+template <int HD, int CT, bool WIDE>
+struct ScaledSweep {
+    static constexpr int NC = HD / 64, DT = HD / 16, NP = WIDE ? 3 : 1;
+
+    bf16x8 q[CT][NC][2][NP];
+    f32x4 o[CT][DT];
+    f32x4 s[CT][4];
+    float m[CT], l[CT];
+    Vec16 k_raw[4][NC], v_raw[DT];
+    float k_scale, v_scale;
+
+    __device__ __forceinline__ void init() {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            m[ct] = NO_SCORE;
+            l[ct] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+
+    static __device__ __forceinline__ void in_pieces(float x, bf16_t (&piece)[NP]) {
+        if constexpr (!WIDE) piece[0] = static_cast<bf16_t>(x);
+        else {
+            // the leading eight bits, the next eight, and the rest: cut off, not rounded, so that nothing overflows
+            auto head_of = [](float y) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & 0xffff0000u); };
+            const float a = head_of(x), r = __builtin_isinf(x) ? 0.0f : x - a, b = head_of(r);
+            piece[0] = static_cast<bf16_t>(a);
+            piece[1] = static_cast<bf16_t>(b);
+            piece[2] = static_cast<bf16_t>(r - b);
+        }
+    }
+
+    // Column ct's query: `row` points at its head's first element (null: no query here). negative: a negative score scale, whose sign the queries take.
+    template <typename T>
+    __device__ __forceinline__ void load_query(int ct, const T* row, int head_size, bool aligned, bool negative, int lane) {
+        const int quarter = lane / 16;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int d = (4 * c + quarter) * 16 + 8 * h;
+                T x[8];
+                if (row != nullptr && d < head_size) {
+                    if (aligned) {
+#pragma unroll
+                        for (int w = 0; w < (int)sizeof(T) / 2; w++) reinterpret_cast<Vec16*>(x)[w] = reinterpret_cast<const Vec16*>(row + d)[w];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] = row[d + i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] = from_float<T>(0.0f);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    bf16_t piece[NP];
+                    in_pieces(negative ? -to_float(x[i]) : to_float(x[i]), piece);
+#pragma unroll
+                    for (int p = 0; p < NP; p++) q[ct][c][h][p][i] = piece[p];
+                }
+            }
+    }
+
+    // Where the lane's block of keys (r / 4) and of values (q) of a tile lie, as numbers of blocks.
+    struct Places {
+        long long k, v;
+    };
+    static __device__ __forceinline__ long long place(int block, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head) {
+        const int shift = planes.page_shift - 4;
+        const unsigned page = min((unsigned)table[block >> shift], (unsigned)planes.num_pages - 1u);   // (nothing a table holds leads out of the pages)
+        return (((long long)page * planes.n_kv_heads + kv_head) << shift) + (block & ((1 << shift) - 1));
+    }
+    static __device__ __forceinline__ Places look_up(const TileRange& range, int tile, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head, int lane) {
+        const int block = range.first_key_of(tile) / BLOCK_TOKENS;
+        return {place(range.stored(block + (lane % 16) / 4), table, planes, kv_head), place(range.stored(block + lane / 16), table, planes, kv_head)};
+    }
+
+    __device__ __forceinline__ void load_keys(const Places& at, const ScaledPlanes& planes, int lane) {
+        const int quarter = lane / 16, r = lane % 16, pieces = planes.head_size / 16;
+        const Vec16* const block = reinterpret_cast<const Vec16*>(planes.k_codes) + at.k * planes.head_size;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < NC; c++)   // (pieces beyond the head's: its last once more, which meet zeros of the query)
+                k_raw[t][c] = block[min(4 * c + quarter, pieces - 1) * 16 + 4 * t + r % 4];
+        k_scale = planes.k_scales[at.k];
+    }
+    __device__ __forceinline__ void load_values(const Places& at, const ScaledPlanes& planes, int lane) {
+        const Vec16* const block = reinterpret_cast<const Vec16*>(planes.v_codes) + at.v * planes.head_size;
+        const int tiles = planes.head_size / 16;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) v_raw[dt] = block[min(dt, tiles - 1) * 16 + lane % 16];
+        v_scale = planes.v_scales[at.v];
+    }
+
+    __device__ __forceinline__ void scores() {
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const bf16x8 keys = eight_numbers(k_raw[t][c].w[2 * h], k_raw[t][c].w[2 * h + 1], k_scale);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                        for (int p = NP - 1; p >= 0; p--) s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, q[ct][c][h][p], s[ct][t], 0, 0, 0);
+                }
+    }
+
+    // Takes the tile's scores and values into the running sums. first_key: of the tile. MASKED: some column does not see some key; a key counts
+    // for column ct if it is at most last[ct] and (at least first[ct] or below keep).
+    template <bool MASKED>
+    __device__ __forceinline__ void take(const ScoreScale& scale, int first_key, const int (&first)[CT], const int (&last)[CT], int keep, int lane) {
+        const int key = first_key + BLOCK_TOKENS * (lane / 16);   // the lane's keys: key + 4 t + i
+        uint32_t seen[CT];
+        bool raise = false;
+        float top[CT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            if (scale.cap > 0.0f) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = s[ct][t][i] * scale.cap_in;
+                        s[ct][t][i] = scale.cap * (WIDE ? tanhf(x) : 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * 2.8853900817779268f)));
+                    }
+            }
+            if constexpr (MASKED) {
+                seen[ct] = 0;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int k = key + 4 * t + i;
+                        const bool counts = k <= last[ct] && (k >= first[ct] || k < keep);
+                        seen[ct] |= counts ? 1u << (4 * t + i) : 0u;
+                        s[ct][t][i] = counts ? s[ct][t][i] : -INFINITY;
+                    }
+            }
+            float best = s[ct][0][0];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) best = fmaxf(best, s[ct][t][i]);
+            top[ct] = scale.cap > 0.0f ? best : best * scale.factor;
+            raise |= top[ct] > m[ct] + SCORE_SLACK;
+        }
+        if (__any(raise)) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                float best = top[ct];
+                best = fmaxf(best, __shfl_xor(best, 16, WAVE));
+                best = fmaxf(best, __shfl_xor(best, 32, WAVE));
+                const float higher = fmaxf(m[ct], best);
+                const float fall = weight_of<WIDE>(m[ct] - higher);
+                m[ct] = higher;
+                l[ct] *= fall;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[ct][dt][i] *= fall;
+            }
+        }
+        bf16x8 weights[CT][2][NP];
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float x = scale.cap > 0.0f ? s[ct][t][i] - m[ct] : WIDE ? s[ct][t][i] * scale.factor - m[ct] : __builtin_fmaf(s[ct][t][i], scale.factor, -m[ct]);
+                    const float p = weight_of<WIDE>(x);
+                    sum += p;
+                    bf16_t piece[NP];
+                    in_pieces(p, piece);
+#pragma unroll
+                    for (int n = 0; n < NP; n++) weights[ct][t / 2][n][4 * (t % 2) + i] = piece[n];
+                }
+            l[ct] += sum;
+        }
+        if constexpr (MASKED) {
+            // Not even a weight of zero silences a NaN: where the tile has any (in places that nothing was written to, or that some column does not
+            // see), they are taken out, and each goes to the columns that see it.
+            uint32_t none = 0;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) none |= not_numbers(v_raw[dt].w[0]) | not_numbers(v_raw[dt].w[1]) | not_numbers(v_raw[dt].w[2]) | not_numbers(v_raw[dt].w[3]);
+            if (__any(none != 0)) {
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    Vec16 ones;
+                    uint32_t some = 0;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t high = not_numbers(v_raw[dt].w[w]) >> 7;   // 1 in each byte that is no number
+                        some |= high;
+                        ones.w[w] = high * 0x38u;                                 // the code of 1
+                        v_raw[dt].w[w] &= ~(high * 0xffu);
+                    }
+                    if (__any(some != 0)) {
+#pragma unroll
+                        for (int ct = 0; ct < CT; ct++) {
+                            f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                bf16x8 sees;
+#pragma unroll
+                                for (int i = 0; i < 8; i++) sees[i] = static_cast<bf16_t>((seen[ct] >> (8 * h + i)) & 1u ? 1.0f : 0.0f);
+                                count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_numbers(ones.w[2 * h], ones.w[2 * h + 1], 1.0f), sees, count, 0, 0, 0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[ct][dt][i] = count[i] > 0.0f ? __builtin_nanf("") : o[ct][dt][i];
+                        }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const bf16x8 values = eight_numbers(v_raw[dt].w[2 * h], v_raw[dt].w[2 * h + 1], v_scale);
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int n = NP - 1; n >= 0; n--) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, weights[ct][h][n], o[ct][dt], 0, 0, 0);
+            }
+    }
+
+    // Tiles tile, tile + step, .. below `end`. all_from / all_to: every column sees the keys all_from .. all_to (beside kept ones).
+    __device__ __forceinline__ void tiles(const TileRange& range, int tile, int step, int end, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head,
+                                          const ScoreScale& scale, const int (&first)[CT], const int (&last)[CT], int all_from, int all_to, int keep, int lane) {
+        if (tile >= end) return;
+        Places at = look_up(range, tile, table, planes, kv_head, lane);
+        load_keys(at, planes, lane);
+        load_values(at, planes, lane);
+        for (; tile < end; tile += step) {
+            const bool more = tile + step < end;
+            if (more) at = look_up(range, tile + step, table, planes, kv_head, lane);
+            scores();
+            if (more) load_keys(at, planes, lane);   // the next tile's, while this one's weights are made
+            const int first_key = range.first_key_of(tile);
+            if (first_key >= all_from && first_key + TILE_KEYS - 1 <= all_to) take<false>(scale, first_key, first, last, keep, lane);
+            else take<true>(scale, first_key, first, last, keep, lane);
+            if (more) load_values(at, planes, lane);
+        }
+    }
+};

@@ -495,8 +495,13 @@ def paged_attention(q, k_pages, v_pages, token_request, positions, block_tables,
     keys in one wave of the kernel for portions).
     ``packed_out``: where the kernel for decoding and short portions runs, the rows come as
     PackedRows (for the output product of few rows that reads them next); elsewhere as ever.
+    Pages may be ``ScaledPages``, keys and values in 8 bits with a scale a block: q is then bfloat16 or float32 whatever they are, and the
+    products are as exact as that type's (what is held in 8 bits is exact in bfloat16).
     ``first_row``: where the rows are a part of a step's batch whose other parts may run at the same time on other
     streams, the place of the first of them in the whole batch (kernels that keep counters per row keep them apart by it)."""
+    if isinstance(k_pages, ScaledPages):
+        return _scaled_attention(q, k_pages, v_pages, token_request, positions, block_tables, n_heads, n_kv_heads, head_size, float(scale), int(window or 0), max_q_len, max_len,
+                                 q_starts, context_lens, out, short_rows, short_requests, packed_out, float(softcap or 0.0), sinks, int(chunk or 0), int(keep_first or 0), bool(wide_out))
     _check_pages(k_pages, v_pages, n_kv_heads, head_size)
     page_size = k_pages.shape[2]
     width = n_heads * head_size
@@ -1463,6 +1468,259 @@ def recurrence(q, k, v, state, q_starts, state_slots, n_heads, dim, vdim, *, gat
     check(library().mllm_recurrence(0 if gated else 1, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), _ptr(gate_in), _ptr(gate_forget),
                                     gate_in.stride(0) if gated else 0, float(cap or 0.0), _ptr(decay), float(q_scale), _ptr(state), state.stride(0), matrices,
                                     matrices + n_heads * dim, _ptr(q_starts), _ptr(state_slots), _ptr(out), out.stride(0), n_requests, n_heads, dim, vdim, _stream()))
+    return out
+
+
+# -- a cache of 8 bits ----------------------------------------------------------------------------------------------------------
+SCALE_BLOCK = 16            # tokens of a head that share a scale
+SCALED_MAX_HEAD = 256
+E4M3 = torch.float8_e4m3fn
+
+
+@dataclass(frozen=True)
+class ScaledPages:
+    """The pages of one cache layer's keys, or of its values, in 8 bits with a scale for every block of SCALE_BLOCK tokens of a head: a number
+    x is held as the code nearest to x / scale, scale the smallest power of two (2^-110 .. 2^118) with 448 scale at least the block's largest
+    magnitude (numbers past 448 * 2^118 are held as that, infinities as NaN).
+
+    ``codes`` (float8_e4m3fn): keys [num_pages, n_kv_heads, page_size / 16, head_size / 16, 16 tokens, 16 elements], values [num_pages,
+    n_kv_heads, page_size / 16, head_size, 16 tokens]: a block lies as the matrix instructions take it (csrc/scaled_blocks.h). ``scales``:
+    float32 [num_pages, n_kv_heads, page_size / 16]. ``scaled_append`` writes them, ``paged_attention`` reads them where it is given them as
+    pages, ``scaled_rows`` gives what they hold. ``shape`` and ``dtype`` are as pages of plain rows have them."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self):
+        codes, scales = self.codes, self.scales
+        _require(isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor), "codes and scales are tensors")
+        _require(codes.dtype == E4M3 and scales.dtype == torch.float32, f"codes are {E4M3} and scales float32, not {codes.dtype} and {scales.dtype}")
+        _require(codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device, "codes and scales are contiguous and lie on one device")
+        _require(codes.dim() in (5, 6) and codes.shape[-1] == SCALE_BLOCK and (codes.dim() == 5 or codes.shape[-2] == SCALE_BLOCK), "codes have neither the shape of keys nor that of values")
+        _require(scales.dim() == 3 and tuple(scales.shape) == tuple(codes.shape[:3]), "one scale a block")
+        page_size, head_size = self.page_size, self.head_size
+        _require(page_size >= SCALE_BLOCK and page_size & (page_size - 1) == 0, f"page size {page_size} is no power of two of at least {SCALE_BLOCK}")
+        _require(codes.shape[0] > 0 and codes.shape[1] > 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD, f"heads of {head_size} are not a multiple of 16 up to {SCALED_MAX_HEAD}")
+
+    @property
+    def is_keys(self) -> bool:
+        return self.codes.dim() == 6
+
+    @property
+    def page_size(self) -> int:
+        return self.codes.shape[2] * SCALE_BLOCK
+
+    @property
+    def head_size(self) -> int:
+        return self.codes.shape[3] * (16 if self.is_keys else 1)
+
+    @property
+    def shape(self) -> tuple:
+        return (self.codes.shape[0], self.codes.shape[1], self.page_size, self.head_size)
+
+    @property
+    def dtype(self):
+        return self.codes.dtype
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def scaled_pages(num_pages: int, n_kv_heads: int, page_size: int, head_size: int, device) -> tuple[ScaledPages, ScaledPages]:
+    """Empty key pages and value pages of 8 bits (zeros, scales of 1)."""
+    _require(page_size >= SCALE_BLOCK and page_size & (page_size - 1) == 0, f"page size {page_size} is no power of two of at least {SCALE_BLOCK}")
+    _require(num_pages > 0 and n_kv_heads > 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD, f"heads of {head_size} are not a multiple of 16 up to {SCALED_MAX_HEAD}")
+    blocks = (num_pages, n_kv_heads, page_size // SCALE_BLOCK)
+    codes = lambda *block: torch.zeros(blocks + block, dtype=torch.uint8, device=device).view(E4M3)
+    scales = lambda: torch.ones(blocks, dtype=torch.float32, device=device)
+    return ScaledPages(codes(head_size // 16, SCALE_BLOCK, 16), scales()), ScaledPages(codes(head_size, SCALE_BLOCK), scales())
+
+
+def _check_scaled(k_pages, v_pages, n_kv_heads: int, head_size: int):
+    if not (isinstance(k_pages, ScaledPages) and isinstance(v_pages, ScaledPages) and k_pages.is_keys and not v_pages.is_keys):
+        raise OperandError("key pages and value pages of 8 bits go together, each in its place")
+    _require(k_pages.shape == v_pages.shape, "key and value pages differ in shape")
+    _require(k_pages.shape[1] == n_kv_heads and k_pages.shape[3] == head_size, "pages do not match the heads")
+    _require(k_pages.codes.is_cuda and v_pages.codes.is_cuda, "the pages are not on the GPU: there is no CPU path")
+
+
+def _one_device(*tensors) -> None:
+    """Kernels run on the current device's stream: what they are given lies there."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise OperandError(f"a tensor on {t.device} meets a kernel on the current device, cuda:{here}")
+
+
+def _strided_rows(t, name: str, width: int) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.shape[1] == width and (t.stride(1) == 1 or width == 1)):
+        raise OperandError(f"{name} must be 2-D on the GPU with {width} contiguous columns")
+    _require(t.stride(0) >= width or t.shape[0] <= 1, f"{name}'s rows overlap")
+
+
+def _rotation(frequencies, dims: int, most: int, pairing: str, name: str):
+    dims = int(dims or 0)
+    _require(pairing in ("half", "neighbours"), f"{name} pair by halves or by neighbours")
+    if frequencies is None or dims == 0:
+        return None, 0
+    _device_tensor(frequencies, f"the frequencies of {name}", torch.float64, 1)
+    _require(dims % 2 == 0 and 0 < dims <= most and frequencies.shape[0] >= dims // 2, f"the rotation does not fit {name}")
+    return frequencies, dims
+
+
+def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_pages, v_pages, slots, positions, n_heads: int, n_kv_heads: int, dim: int, vdim: int, *, q_gain=None,
+                  k_gain=None, unit: bool = False, eps: float = 0.0, frequencies=None, rot_dims: int = 0, pairing: str = "half", v_frequencies=None, v_rot_dims: int = 0,
+                  v_pairing: str = "half"):
+    """The row-wise work between a mixer's input product and its attention over pages of 8 bits (``ScaledPages``), in one kernel. ``rows``
+    (float32 or bfloat16; rows may be strided): the queries [n_heads, dim] at column ``q_at`` (None: no queries are made), the keys [n_kv_heads, dim]
+    at ``k_at`` and the values [n_kv_heads, vdim] at ``v_at`` (both None: the layer reads pages another layer keeps, and only its queries are
+    made). Queries and keys are RMS-normed over their ``dim`` elements where they have a gain ([dim], float32) or, with ``unit``, without one; their
+    first ``rot_dims`` elements turn in pairs by position * frequencies[pair] (float64, the angle in 64-bit), pairs (i, i + rot_dims / 2) with ``pairing``
+    "half" or (2i, 2i + 1) with "neighbours"; ``v_frequencies``, ``v_rot_dims`` and ``v_pairing`` turn the values likewise.
+
+    Keys and values of row r go to slots[r] = page * page_size + offset (negative, or behind the pages: nowhere). Rows whose slots fall into
+    one block are neighbours and follow each other, as a request's tokens do, and no slot is named twice. A block whose first token
+    is written begins afresh; a block that is carried on keeps its scale or, if the new rows need a larger one, is taken to that (its earlier
+    tokens' codes rounded again). Tokens of a block behind those written stay as they are.
+
+    Returns the queries [rows, n_heads * head_size] in the rows' type, zeros behind their ``dim`` elements (None without ``q_at``)."""
+    _, _, page_size, head_size = k_pages.shape
+    _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
+    _require(isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _DTYPE_CODE and (rows.stride(1) == 1 or rows.shape[1] == 1),
+             "the rows must be float32 or bfloat16 GPU rows with contiguous columns")
+    n, width = rows.shape
+    _require(rows.stride(0) >= width or n <= 1, "the rows overlap")
+    keeps, makes = k_at is not None, q_at is not None
+    _require(keeps == (v_at is not None), "keys and values are kept together")
+    _require(keeps or makes, "neither queries nor keys")
+    _require(0 < dim <= head_size and 0 < vdim <= head_size, "the pages' heads are too small")
+    _require(n_heads > 0 and n_kv_heads > 0, "heads are at least one")
+    _require(not makes or (0 <= q_at and q_at + n_heads * dim <= width), "the queries lie beyond the rows")
+    _require(not keeps or (0 <= k_at and k_at + n_kv_heads * dim <= width and 0 <= v_at and v_at + n_kv_heads * vdim <= width), "keys or values lie beyond the rows")
+    for gain, name in ((q_gain, "q_gain"), (k_gain, "k_gain")):
+        if gain is not None:
+            _device_tensor(gain, name, torch.float32, 1)
+            _require(gain.shape[0] == dim, f"{name} does not match the heads")
+    frequencies, rot_dims = _rotation(frequencies, rot_dims, dim, pairing, "queries and keys")
+    v_frequencies, v_rot_dims = _rotation(v_frequencies, v_rot_dims, vdim, v_pairing, "values")
+    _device_tensor(positions, "positions", torch.int32, 1)
+    _require(positions.shape[0] >= n, "fewer positions than rows")
+    if keeps:
+        _device_tensor(slots, "slots", torch.int32, 1)
+        _require(slots.shape[0] >= n, "fewer slots than rows")
+        _require(k_pages.shape[0] * page_size <= 2**31, "the pages hold more tokens than a slot can name")
+    _one_device(rows, k_pages.codes, v_pages.codes, positions, slots if keeps else None, q_gain, k_gain, frequencies, v_frequencies)
+    q = torch.empty((n, n_heads * head_size), dtype=rows.dtype, device=rows.device) if makes else None
+    check(library().mllm_scaled_append(_ptr(rows), rows.stride(0), int(q_at) if makes else -1, int(k_at) if keeps else -1, int(v_at) if keeps else -1, _ptr(q_gain), _ptr(k_gain),
+                                       float(eps), int(bool(unit)), _ptr(frequencies), rot_dims, int(pairing == "neighbours"), _ptr(v_frequencies), v_rot_dims,
+                                       int(v_pairing == "neighbours"), _ptr(positions), _ptr(slots if keeps else None), _ptr(q), _ptr(k_pages.codes), _ptr(k_pages.scales),
+                                       _ptr(v_pages.codes), _ptr(v_pages.scales), k_pages.shape[0], n, n_heads, n_kv_heads, int(dim), int(vdim), head_size, page_size,
+                                       _code(rows.dtype), _stream()))
+    return q
+
+
+def scaled_rows(k_pages, v_pages, slots, out_dtype=torch.bfloat16):
+    """What pages of 8 bits hold at ``slots`` (int32): (keys, values), each [len(slots), n_kv_heads, head_size] of ``out_dtype`` (bfloat16 holds them
+    exactly); zeros where a slot is negative or lies behind the pages."""
+    num_pages, n_kv_heads, page_size, head_size = k_pages.shape
+    _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
+    _device_tensor(slots, "slots", torch.int32, 1)
+    _one_device(k_pages.codes, v_pages.codes, slots)
+    n = slots.shape[0]
+    k, v = (torch.empty((n, n_kv_heads, head_size), dtype=out_dtype, device=slots.device) for _ in range(2))
+    check(library().mllm_scaled_rows(_ptr(k_pages.codes), _ptr(k_pages.scales), _ptr(v_pages.codes), _ptr(v_pages.scales), _ptr(slots), _ptr(k), _ptr(v), num_pages, n,
+                                     n_kv_heads, head_size, page_size, _code(out_dtype), _stream()))
+    return k, v
+
+
+SCALED_TILE = 64            # keys a wave takes at a time
+SCALED_SHORT = 8            # portions up to so many tokens go row by row
+
+
+def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int) -> tuple[int, int, int]:
+    """(waves a block, tiles a run, runs) for the rows kernel over pages of 8 bits: ``blocks`` (row, head group) pairs, each with up to ``tiles`` tiles of
+    keys, ``columns`` heads of ``head_size`` a block."""
+    most = 1024 // (64 if head_size <= 64 else 128 if head_size <= 128 else 256)
+    while most > 1 and most * columns * (head_size + 4) * 4 > 65536:
+        most //= 2
+    run = tiles
+    while run > most and blocks * -(-tiles // run) < 512:
+        run = -(-run // 2)
+    waves = 1
+    while waves < most and waves < run and (blocks * -(-tiles // run)) * waves < 4096:
+        waves *= 2
+    return waves, run, -(-tiles // run)
+
+
+def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_tables, n_heads, n_kv_heads, head_size, scale, window, max_q_len, max_len, q_starts, context_lens, out,
+                      short_rows, short_requests, packed_out, softcap, sinks, chunk, keep_first, wide_out):
+    """``paged_attention`` over pages of 8 bits: rows by themselves (decoding, short portions, batches without the shape of portions) a block per
+    row and group of heads; portions a block per head and tile of rows."""
+    _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
+    num_pages, _, page_size, _ = k_pages.shape
+    _require(n_heads > 0 and n_heads % n_kv_heads == 0, f"{n_heads} heads do not divide into {n_kv_heads} key/value heads")
+    width = n_heads * head_size
+    _strided_rows(q, "q", width)
+    if q.dtype not in _DTYPE_CODE:
+        raise OperandError(f"no kernel for element type {q.dtype}")
+    n = q.shape[0]
+    _device_tensor(block_tables, "block_tables", torch.int32, 2)
+    _require(block_tables.shape[0] > 0 and block_tables.shape[1] > 0, "block tables without entries")
+    _require(window >= 0 and chunk >= 0 and not (chunk and window), "the keys a row sees are bounded by a window or by chunks, not both")
+    keep = keep_first if window else 0
+    _require(keep >= 0, "kept first keys are a number of them")
+    _require(not (wide_out and packed_out), "rows in the packed layout leave in the queries' type")
+    if sinks is not None:
+        _device_tensor(sinks, "sinks", torch.float32, 1)
+        _require(sinks.shape[0] == n_heads, "one sink a head")
+    out_dtype = torch.float32 if wide_out else q.dtype
+    if out is None:
+        out = torch.empty((n, width), dtype=out_dtype, device=q.device)
+    _strided_rows(out, "out", width)
+    _require(out.dtype == out_dtype and out.shape[0] == n, "out has the wrong shape or type")
+    _device_tensor(token_request, "token_request", torch.int32, 1)
+    _device_tensor(positions, "positions", torch.int32, 1)
+    _require(token_request.shape[0] >= n and positions.shape[0] >= n, "fewer positions than rows")
+    _one_device(q, out, k_pages.codes, v_pages.codes, token_request, positions, block_tables, sinks, q_starts, context_lens)
+    lib = library()
+    if n == 0:
+        return out
+    reach = block_tables.shape[1] * page_size
+    pages = (_ptr(k_pages.codes), _ptr(k_pages.scales), _ptr(v_pages.codes), _ptr(v_pages.scales))
+
+    def rows_alone(count, into, packed):
+        span = min(window + keep if window else chunk or reach, reach)
+        tiles = -(-span // SCALED_TILE) + (2 if window or chunk else 0)
+        sets = -(-(n_heads // n_kv_heads) // 16)
+        longest = tiles if max_len is None else max(1, min(tiles, -(-int(max_len) // SCALED_TILE)))
+        waves, run, runs = scaled_cut(count * n_kv_heads * sets, longest, head_size, min(16, n_heads // n_kv_heads))
+        parts = torch.empty((count, n_heads, runs, head_size + 2), dtype=torch.float32, device=q.device) if runs > 1 else None
+        check(lib.mllm_scaled_attention_rows(_ptr(q), q.stride(0), *pages, _ptr(into), width if packed else into.stride(0), _ptr(token_request), _ptr(positions),
+                                             _ptr(block_tables), block_tables.shape[1], block_tables.shape[0], num_pages, count, n_heads, n_kv_heads, head_size, page_size, window,
+                                             scale, _code(q.dtype), softcap, _ptr(sinks), chunk, keep, int(wide_out), int(packed), waves, run, runs, _ptr(parts), _stream()))
+
+    portions = max_q_len is not None and max_q_len > SCALED_SHORT and q_starts is not None and context_lens is not None
+    if not portions:
+        if packed_out:
+            result = empty_packed_rows(n, width, q.dtype, q.device)
+            rows_alone(n, result.data, True)
+            return result
+        rows_alone(n, out, False)
+        return out
+    _device_tensor(q_starts, "q_starts", torch.int32, 1)
+    _device_tensor(context_lens, "context_lens", torch.int32, 1)
+    n_requests = context_lens.shape[0]
+    _require(q_starts.shape[0] == n_requests + 1, "q_starts must have one entry more than context_lens")
+    _require(block_tables.shape[0] >= n_requests, "fewer block tables than requests")
+    skipped = 0
+    if short_rows is not None and short_requests is not None and 0 < short_rows < n:
+        _require(0 < short_requests < n_requests, "short_requests does not cut the batch in two")
+        rows_alone(int(short_rows), out, False)
+        skipped = int(short_requests)
+    check(lib.mllm_scaled_attention_tiles(_ptr(q), q.stride(0), *pages, _ptr(out), out.stride(0), _ptr(q_starts[skipped:]), _ptr(context_lens[skipped:]), _ptr(block_tables[skipped:]),
+                                          block_tables.shape[1], n_requests - skipped, num_pages, n, int(max_q_len), n_heads, n_kv_heads, head_size, page_size, window, scale,
+                                          _code(q.dtype), softcap, _ptr(sinks), chunk, keep, int(wide_out), _stream()))
     return out
 
 

@@ -1,0 +1,71 @@
+"""Pages of 8 bits: what the calls refuse, and the bookkeeping that needs no GPU."""
+
+import pytest
+import torch
+
+from mini_llm_amd.ops import kernels as K
+
+
+def codes(*shape):
+    return torch.zeros(shape, dtype=torch.uint8).view(torch.float8_e4m3fn)
+
+
+def test_shapes_of_pages():
+    k, v = K.scaled_pages(3, 2, 64, 48, "cpu")
+    assert k.shape == v.shape == (3, 2, 64, 48) and k.is_keys and not v.is_keys
+    assert k.codes.shape == (3, 2, 4, 3, 16, 16) and v.codes.shape == (3, 2, 4, 48, 16) and k.scales.shape == (3, 2, 4)
+    assert k.dtype == torch.float8_e4m3fn and bool((v.scales == 1).all())
+
+
+@pytest.mark.parametrize("args", [(0, 1, 16, 16), (1, 0, 16, 16), (1, 1, 8, 16), (1, 1, 48, 16), (1, 1, 16, 24), (1, 1, 16, 0), (1, 1, 16, 272)])
+def test_pages_that_cannot_be(args):
+    with pytest.raises(K.OperandError):
+        K.scaled_pages(*args, "cpu")
+
+
+@pytest.mark.parametrize("make", [
+    lambda: (torch.zeros((1, 1, 1, 1, 16, 16)), torch.ones((1, 1, 1))),
+    lambda: (codes(1, 1, 1, 1, 16, 16), torch.ones((1, 1, 1), dtype=torch.float64)),
+    lambda: (codes(1, 1, 1, 1, 16, 16), torch.ones((1, 1, 2))),
+    lambda: (codes(1, 1, 1, 16), torch.ones((1, 1, 1))),
+    lambda: (codes(1, 1, 1, 16, 8), torch.ones((1, 1, 1))),
+    lambda: (codes(1, 1, 3, 16, 16), torch.ones((1, 1, 3))),
+    lambda: (codes(1, 1, 1, 24, 16), torch.ones((1, 1, 1))),
+    lambda: (codes(1, 2, 3, 16, 16).transpose(1, 2), torch.ones((1, 3, 2))),
+    lambda: ("codes", torch.ones((1, 1, 1)))])
+def test_codes_and_scales_that_do_not_fit(make):
+    with pytest.raises(K.OperandError):
+        K.ScaledPages(*make())
+
+
+def test_the_cpu_is_refused():
+    k, v = K.scaled_pages(1, 1, 16, 16, "cpu")
+    ints = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(K.OperandError, match="GPU"):
+        K.scaled_append(torch.zeros((1, 48)), 0, 16, 32, k, v, ints, ints, 1, 1, 16, 16)
+    with pytest.raises(K.OperandError, match="GPU"):
+        K.paged_attention(torch.zeros((1, 16)), k, v, ints, ints, ints[None], 1, 1, 16, 0.25)
+    with pytest.raises(K.OperandError, match="GPU"):
+        K.scaled_rows(k, v, ints)
+
+
+def test_planes_in_the_wrong_place_are_refused():
+    k, v = K.scaled_pages(1, 1, 16, 16, "cpu")
+    plain = torch.zeros((1, 1, 16, 16))
+    ints = torch.zeros(1, dtype=torch.int32)
+    for pair in ((v, k), (k, k), (k, plain)):
+        with pytest.raises(K.OperandError):
+            K.paged_attention(torch.zeros((1, 16)), *pair, ints, ints, ints[None], 1, 1, 16, 0.25)
+        with pytest.raises(K.OperandError):
+            K.scaled_append(torch.zeros((1, 48)), 0, 16, 32, *pair, ints, ints, 1, 1, 16, 16)
+    with pytest.raises(K.OperandError):
+        K.scaled_rows(k, K.scaled_pages(2, 1, 16, 16, "cpu")[1], ints)
+
+
+@pytest.mark.parametrize("blocks", [1, 12, 100, 1000, 100000])
+@pytest.mark.parametrize("tiles", [1, 2, 16, 17, 500, 16384])
+@pytest.mark.parametrize("head_size,columns", [(16, 1), (64, 16), (128, 4), (128, 16), (256, 1), (256, 16)])
+def test_cuts_fit_what_the_kernel_takes(blocks, tiles, head_size, columns):
+    waves, run, runs = K.scaled_cut(blocks, tiles, head_size, columns)
+    assert 1 <= waves <= 16 and waves & (waves - 1) == 0 and waves * columns * (head_size + 4) * 4 <= 65536
+    assert run >= 1 and run * runs >= tiles and run * (runs - 1) < tiles and 1 <= runs <= 65535
