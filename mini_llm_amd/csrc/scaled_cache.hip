@@ -4,6 +4,8 @@
 
 namespace {
 
+constexpr int APPEND_BLOCKS = 1024;   // blocks of threads that a call is shared among, if it has the heads for them
+
 // What is done to the heads of one kind on their way.
 struct Turn {
     const double* frequencies;   // null: nothing is turned
@@ -28,7 +30,7 @@ struct AppendArguments {
     uint8_t* v_codes;
     float* v_scales;
     long long n_slots;
-    int n_rows, n_heads, n_kv_heads, dim, vdim, head_size, page_shift;
+    int n_rows, n_heads, n_kv_heads, dim, vdim, head_size, page_shift, q_wide;
 };
 
 // cos and sin of position x frequency to the last bits of 64: the turns are taken off in quarters, and what is left, at most pi / 4, goes
@@ -58,10 +60,355 @@ __device__ __forceinline__ float sticky(double x) {
     return __builtin_bit_cast(float, bits | 1u);
 }
 
-// A block: a run of rows after another (those that begin in its `per` rows), each by all its waves: the cosines and sines of the run's
-// positions once for all heads, then a head's keys or values of the run at a time, or a row's query head, by a wave. A lane has
-// E elements of the head, 64 apart.
+// A run of rows that fall into one block, as a block of threads takes it.
+struct Run {
+    int first, count;      // rows first .. first + count - 1
+    bool kept;             // whether they go anywhere
+    int lead;              // the first one's token in its block
+    size_t block_in_head;  // the block: of head 0, and how far the next head's lies
+    size_t head_blocks;
+};
+
+// What becomes of a block's scale: `exponent` holds the new rows and what the block holds in front of them.
+struct BlockScale {
+    int exponent;
+    float inverse, factor;   // of new numbers; of codes that the block holds
+    bool grown;
+    __device__ __forceinline__ BlockScale(float largest, int lead, float held) {
+        const int old = lead > 0 ? scale_exponent(held) : SCALE_LOW;
+        exponent = max(old, needed_exponent(largest));
+        inverse = two_to(-exponent);
+        factor = exponent - old < 126 ? two_to(old - exponent) : 0.0f;
+        grown = lead > 0 && exponent > old;
+    }
+};
+
+// Where the pair of element d lies, its number, and whether d is the first of the two.
+__device__ __forceinline__ int partner_of(const Turn& turn, int d, int& pair, bool& is_first) {
+    const int half = turn.dims / 2;
+    pair = turn.neighbours ? d / 2 : d % half;
+    is_first = turn.neighbours ? d % 2 == 0 : d < half;
+    return turn.neighbours ? d ^ 1 : is_first ? d + half : d - half;
+}
+
+// The value of a pair's element, in 64 bits and rounded once.
+__device__ __forceinline__ float turned_once(float value, float other, bool is_first, double2 cs) {
+    return sticky(fma((double)value, cs.x, (double)other * (is_first ? -cs.y : cs.y)));
+}
+
+// The keys that a block holds in front of the new ones, taken to its new scale: (head_size / 16) x 16 pieces of 16 bytes.
+__device__ __forceinline__ void rescale_keys(uint8_t* codes, int head_size, int lead, float factor, int lane) {
+    for (int i = lane; i < head_size; i += WAVE)
+        if (i % BLOCK_TOKENS < lead) {
+            Vec16* const at = reinterpret_cast<Vec16*>(codes) + i;
+            Vec16 piece = *at;
+#pragma unroll
+            for (int w = 0; w < 4; w++) piece.w[w] = rescaled_codes(piece.w[w], factor);
+            *at = piece;
+        }
+}
+
+// A head's values of a run, by a wave: a lane has elements lane, lane + 64, .. of every row, so that what it makes of one is the 16 tokens'
+// codes that lie together.
 template <typename T, int E>
+__device__ __forceinline__ void append_values(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+    const size_t block = run.block_in_head + head * run.head_blocks;
+    uint8_t* const codes = a.v_codes + block * BLOCK_TOKENS * a.head_size;
+    const T* const from = static_cast<const T*>(a.rows) + (size_t)run.first * a.stride + a.v_at + head * a.vdim;
+    const float held = a.v_scales[block];
+    float x[BLOCK_TOKENS][E];
+    Vec16 piece[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int d = lane + e * WAVE;
+#pragma unroll
+        for (int t = 0; t < BLOCK_TOKENS; t++) x[t][e] = t < run.count && d < a.vdim ? to_float(from[t * a.stride + d]) : 0.0f;
+        piece[e] = Vec16{{0u, 0u, 0u, 0u}};
+        if (run.count < BLOCK_TOKENS && d < a.head_size) piece[e] = *reinterpret_cast<const Vec16*>(codes + d * BLOCK_TOKENS);
+    }
+    if (pairs) {
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int d = lane + e * WAVE;
+            if (d < a.v_turn.dims) {
+                int pair;
+                bool is_first;
+                const int other = partner_of(a.v_turn, d, pair, is_first);
+#pragma unroll
+                for (int t = 0; t < BLOCK_TOKENS; t++)
+                    if (t < run.count) x[t][e] = turned_once(x[t][e], to_float(from[t * a.stride + other]), is_first, turns[t * pairs + pair]);
+            }
+        }
+    }
+    float largest = 0.0f;
+#pragma unroll
+    for (int t = 0; t < BLOCK_TOKENS; t++)
+#pragma unroll
+        for (int e = 0; e < E; e++) largest = fmaxf(largest, counted_magnitude(x[t][e]));
+    const BlockScale scale(wave_max_total(largest), run.lead, held);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int d = lane + e * WAVE;
+        uint32_t fresh[4];   // this run's codes from token 0 on, then moved to where they belong
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            fresh[w] = four_codes(ready_for_code(x[4 * w][e], scale.inverse), ready_for_code(x[4 * w + 1][e], scale.inverse), ready_for_code(x[4 * w + 2][e], scale.inverse),
+                                  ready_for_code(x[4 * w + 3][e], scale.inverse));
+        if (run.count < BLOCK_TOKENS) {
+            const uint64_t low = fresh[0] | (uint64_t)fresh[1] << 32, high = fresh[2] | (uint64_t)fresh[3] << 32;
+            const int bits = 8 * run.lead;   // the run's codes moved up by `lead` bytes of 16
+            const uint64_t up_low = bits < 64 ? low << bits : 0, up_high = bits == 0 ? high : bits < 64 ? high << bits | low >> (64 - bits) : bits == 64 ? low : low << (bits - 64);
+            auto bytes_from = [](int n) { return n <= 0 ? ~0ull : n >= 8 ? 0ull : ~0ull << (8 * n); };   // bytes n .. 7
+            const int end = run.lead + run.count;
+            const uint64_t mine_low = bytes_from(run.lead) & ~bytes_from(end), mine_high = bytes_from(run.lead - 8) & ~bytes_from(end - 8);
+            const uint64_t old_low = ~bytes_from(run.lead), old_high = ~bytes_from(run.lead - 8);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const int shift = 32 * (w & 1);
+                const uint32_t mine = (uint32_t)((w < 2 ? mine_low : mine_high) >> shift), old = (uint32_t)((w < 2 ? old_low : old_high) >> shift);
+                const uint32_t moved = (uint32_t)((w < 2 ? up_low : up_high) >> shift), was = piece[e].w[w];
+                const uint32_t rescaled = scale.grown ? rescaled_codes(was, scale.factor) : was;
+                piece[e].w[w] = (moved & mine) | (rescaled & old) | (was & ~(mine | old));
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < 4; w++) piece[e].w[w] = fresh[w];
+        }
+        if (d < a.head_size) *reinterpret_cast<Vec16*>(codes + d * BLOCK_TOKENS) = piece[e];
+    }
+    if (lane == 0) a.v_scales[block] = two_to(scale.exponent);
+}
+
+// A head's queries or keys of a run, by a wave, eight elements at a time: lane = 16 u + t has of row t the pieces of unit 4 e + u, two of
+// eight elements each that turn with each other (or lie side by side, where nothing turns or neighbours do).
+template <typename T, int E, bool KEYS>
+struct HeadPieces {
+    float x[E][2][8];
+
+    // where the unit's two pieces begin
+    static __device__ __forceinline__ void pieces_of(const Turn& turn, int unit, int& first, int& second) {
+        const bool apart = turn.frequencies && !turn.neighbours && 16 * unit < turn.dims;
+        first = apart ? 8 * unit : 16 * unit;
+        second = apart ? 8 * unit + turn.dims / 2 : 16 * unit + 8;
+    }
+
+    __device__ __forceinline__ void load(const AppendArguments& a, const Run& run, int column, const float* gain, const double2* turns, int pairs, int lane) {
+        const int token = lane % 16;
+        const T* const from = static_cast<const T*>(a.rows) + (size_t)(run.first + (token < run.count ? token : 0)) * a.stride + column;
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int unit = 4 * e + lane / 16;
+            int at[2];
+            pieces_of(a.turn, unit, at[0], at[1]);
+            const bool there = token < run.count && 16 * unit < a.dim;
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                Vec16 raw[sizeof(T) / 2];
+#pragma unroll
+                for (int w = 0; w < (int)sizeof(T) / 2; w++) raw[w] = there ? reinterpret_cast<const Vec16*>(from + at[p])[w] : Vec16{{0u, 0u, 0u, 0u}};
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[e][p][i] = to_float(reinterpret_cast<const T*>(raw)[i]);
+            }
+        }
+        if (gain != nullptr || a.unit) {
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) sum += x[e][p][i] * x[e][p][i];
+            sum += __shfl_xor(sum, 16, WAVE);   // the row's other units
+            sum += __shfl_xor(sum, 32, WAVE);
+            const float factor = rsqrtf(sum / (float)a.dim + a.eps);
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const int unit = 4 * e + lane / 16;
+                int at[2];
+                pieces_of(a.turn, unit, at[0], at[1]);
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[e][p][i] *= factor * (gain != nullptr && 16 * unit < a.dim ? gain[at[p] + i] : 1.0f);
+            }
+        }
+        if (!pairs) return;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int unit = 4 * e + lane / 16;
+            if (16 * unit >= a.turn.dims || token >= run.count) continue;
+            const double2* const mine = turns + token * pairs;
+            if (a.turn.neighbours) {
+#pragma unroll
+                for (int p = 0; p < 2; p++)
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) turn_pair(x[e][p][i], x[e][p][i + 1], mine[8 * unit + 4 * p + i / 2]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) turn_pair(x[e][0][i], x[e][1][i], mine[8 * unit + i]);
+            }
+        }
+    }
+
+    static __device__ __forceinline__ void turn_pair(float& u, float& v, double2 cs) {
+        if constexpr (KEYS) {
+            const float a = turned_once(u, v, true, cs), b = turned_once(v, u, false, cs);
+            u = a, v = b;
+        } else {
+            const float c = (float)cs.x, s = (float)cs.y, a = u * c - v * s, b = v * c + u * s;
+            u = a, v = b;
+        }
+    }
+};
+
+template <typename O>
+__device__ __forceinline__ void store_eight(O* to, const float (&x)[8]) {
+    Vec16 raw[sizeof(O) / 2];
+#pragma unroll
+    for (int i = 0; i < 8; i++) reinterpret_cast<O*>(raw)[i] = from_float<O>(x[i]);
+#pragma unroll
+    for (int w = 0; w < (int)sizeof(O) / 2; w++) reinterpret_cast<Vec16*>(to)[w] = raw[w];
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void queries_in_pieces(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+    HeadPieces<T, E, false> pieces;
+    pieces.load(a, run, a.q_at + head * a.dim, a.q_gain, turns, pairs, lane);
+    const int token = lane % 16;
+    if (token >= run.count) return;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int unit = 4 * e + lane / 16;
+        if (16 * unit >= a.head_size) continue;
+        int at[2];
+        pieces.pieces_of(a.turn, unit, at[0], at[1]);
+        const size_t to = ((size_t)(run.first + token) * a.n_heads + head) * a.head_size;
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            if (a.q_wide) store_eight(static_cast<float*>(a.q_out) + to + at[p], pieces.x[e][p]);
+            else store_eight(static_cast<bf16_t*>(a.q_out) + to + at[p], pieces.x[e][p]);
+        }
+    }
+}
+
+template <typename T, int E>
+__device__ __forceinline__ void keys_in_pieces(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+    const size_t block = run.block_in_head + head * run.head_blocks;
+    uint8_t* const codes = a.k_codes + block * BLOCK_TOKENS * a.head_size;
+    const float held = a.k_scales[block];
+    HeadPieces<T, E, true> pieces;
+    pieces.load(a, run, a.k_at + head * a.dim, a.k_gain, turns, pairs, lane);
+    float largest = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) largest = fmaxf(largest, lane % 16 < run.count ? counted_magnitude(pieces.x[e][p][i]) : 0.0f);
+    const BlockScale scale(wave_max_total(largest), run.lead, held);
+    if (scale.grown) rescale_keys(codes, a.head_size, run.lead, scale.factor, lane);
+    const int token = lane % 16;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int unit = 4 * e + lane / 16;
+        if (16 * unit >= a.head_size || token >= run.count) continue;
+        int at[2];
+        pieces.pieces_of(a.turn, unit, at[0], at[1]);
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            float ready[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) ready[i] = ready_for_code(pieces.x[e][p][i], scale.inverse);
+            const uint2 eight = make_uint2(four_codes(ready[0], ready[1], ready[2], ready[3]), four_codes(ready[4], ready[5], ready[6], ready[7]));
+            *reinterpret_cast<uint2*>(codes + ((at[p] / 16) * BLOCK_TOKENS + run.lead + token) * 16 + at[p] % 16) = eight;
+        }
+    }
+    if (lane == 0) a.k_scales[block] = two_to(scale.exponent);
+}
+
+// The same an element a lane, for heads and places that are no whole pieces: a row's query head ..
+template <typename T, int E>
+__device__ __forceinline__ void query_by_elements(const AppendArguments& a, const Run& run, int row, int head, const double2* turns, int pairs, int lane) {
+    const T* const from = static_cast<const T*>(a.rows) + (size_t)(run.first + row) * a.stride + a.q_at + head * a.dim;
+    const bool normed = a.q_gain != nullptr || a.unit;
+    float x[E], factor = 1.0f, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        x[e] = lane + e * WAVE < a.dim ? to_float(from[lane + e * WAVE]) : 0.0f;
+        sum += x[e] * x[e];
+    }
+    if (normed) factor = rsqrtf(wave_total(sum) / (float)a.dim + a.eps);
+    auto weighted = [&](float value, int d) { return normed ? value * (factor * (a.q_gain ? a.q_gain[d] : 1.0f)) : value; };
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int d = lane + e * WAVE;
+        float value = d < a.dim ? weighted(x[e], d) : 0.0f;
+        if (pairs && d < a.turn.dims) {
+            int pair;
+            bool is_first;
+            const int other = partner_of(a.turn, d, pair, is_first);
+            const double2 cs = turns[row * pairs + pair];
+            value = value * (float)cs.x + weighted(to_float(from[other]), other) * (is_first ? -(float)cs.y : (float)cs.y);
+        }
+        const size_t to = ((size_t)(run.first + row) * a.n_heads + head) * a.head_size + d;
+        if (d < a.head_size) {
+            if (a.q_wide) static_cast<float*>(a.q_out)[to] = value;
+            else static_cast<bf16_t*>(a.q_out)[to] = from_float<bf16_t>(value);
+        }
+    }
+}
+
+// .. and a head's keys of a run.
+template <typename T, int E>
+__device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+    const size_t block = run.block_in_head + head * run.head_blocks;
+    uint8_t* const codes = a.k_codes + block * BLOCK_TOKENS * a.head_size;
+    const T* const from = static_cast<const T*>(a.rows) + (size_t)run.first * a.stride + a.k_at + head * a.dim;
+    const bool normed = a.k_gain != nullptr || a.unit;
+    const float held = a.k_scales[block];
+    float x[BLOCK_TOKENS][E], largest = 0.0f;
+#pragma unroll
+    for (int t = 0; t < BLOCK_TOKENS; t++) {
+        float factor = 1.0f, sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            x[t][e] = t < run.count && lane + e * WAVE < a.dim ? to_float(from[t * a.stride + lane + e * WAVE]) : 0.0f;
+            sum += x[t][e] * x[t][e];
+        }
+        if (normed && t < run.count) factor = rsqrtf(wave_total(sum) / (float)a.dim + a.eps);
+        auto weighted = [&](float value, int d) { return normed ? value * (factor * (a.k_gain ? a.k_gain[d] : 1.0f)) : value; };
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int d = lane + e * WAVE;
+            if (t < run.count && d < a.dim) {
+                float value = weighted(x[t][e], d);
+                if (pairs && d < a.turn.dims) {
+                    int pair;
+                    bool is_first;
+                    const int other = partner_of(a.turn, d, pair, is_first);
+                    value = turned_once(value, weighted(to_float(from[t * a.stride + other]), other), is_first, turns[t * pairs + pair]);
+                }
+                x[t][e] = value;
+                largest = fmaxf(largest, counted_magnitude(value));
+            }
+        }
+    }
+    const BlockScale scale(wave_max_total(largest), run.lead, held);
+    if (scale.grown) rescale_keys(codes, a.head_size, run.lead, scale.factor, lane);
+#pragma unroll
+    for (int t = 0; t < BLOCK_TOKENS; t++)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int d = lane + e * WAVE;
+            if (t < run.count && d < a.head_size)
+                codes[((d / 16) * BLOCK_TOKENS + run.lead + t) * 16 + d % 16] = (uint8_t)four_codes(ready_for_code(x[t][e], scale.inverse), 0.0f, 0.0f, 0.0f);
+        }
+    if (lane == 0) a.k_scales[block] = two_to(scale.exponent);
+}
+
+// A block of threads: a run of rows after another (those that begin in its `per` rows). The cosines and sines of the run's positions are made
+// once for all heads; then every wave takes heads: keys, values, queries.
+template <typename T, int E, bool PIECES>
 __global__ __launch_bounds__(256) void scaled_append_kernel(AppendArguments a, int per) {
     extern __shared__ double2 turns[];   // [16][pairs] of queries and keys, then of values
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, waves = blockDim.x / WAVE;
@@ -70,179 +417,53 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(AppendArguments a, i
     uint32_t begins = keeps ? run_begins(a.slots, window, a.n_rows, a.n_slots, lane) : 0xffffffffu;
     const int pairs = a.turn.frequencies ? a.turn.dims / 2 : 0, v_pairs = a.v_turn.frequencies && keeps ? a.v_turn.dims / 2 : 0;
     double2* const v_turns = turns + BLOCK_TOKENS * pairs;
-    const T* rows = static_cast<const T*>(a.rows);
 
     while (begins) {
         const int at = __builtin_ctz(begins);
-        const int first = window + at;
-        if (at >= per || first >= a.n_rows) return;
+        Run run;
+        run.first = window + at;
+        if (at >= per || run.first >= a.n_rows) return;
         begins &= begins - 1;
-        const int count = min((begins ? __builtin_ctz(begins) : 32) - at, a.n_rows - first);   // at most 16
-        const int slot = keeps ? a.slots[first] : -1;
-        const bool kept = slot >= 0 && slot < a.n_slots;
+        run.count = min((begins ? __builtin_ctz(begins) : 32) - at, a.n_rows - run.first);   // at most 16
+        const int slot = keeps ? a.slots[run.first] : -1;
+        run.kept = slot >= 0 && slot < a.n_slots;
+        run.lead = slot & (BLOCK_TOKENS - 1);
+        run.head_blocks = (size_t)1 << (a.page_shift - 4);
+        run.block_in_head = run.kept ? (((size_t)(slot >> a.page_shift) * a.n_kv_heads) << (a.page_shift - 4)) + ((slot & ((1 << a.page_shift) - 1)) / BLOCK_TOKENS) : 0;
 
-        for (int i = threadIdx.x; i < count * (pairs + v_pairs); i += blockDim.x) {
-            const bool of_value = i >= count * pairs;
-            const int j = of_value ? i - count * pairs : i, n = of_value ? v_pairs : pairs;
-            double c, s;
-            turn_of(a.positions[first + j / n], (of_value ? a.v_turn : a.turn).frequencies[j % n], c, s);
-            (of_value ? v_turns : turns)[j] = make_double2(c, s);
+        if (pairs + v_pairs) {
+            for (int i = threadIdx.x; i < run.count * (pairs + v_pairs); i += blockDim.x) {
+                const bool of_value = i >= run.count * pairs;
+                const int j = of_value ? i - run.count * pairs : i, n = of_value ? v_pairs : pairs;
+                double c, s;
+                turn_of(a.positions[run.first + j / n], (of_value ? a.v_turn : a.turn).frequencies[j % n], c, s);
+                (of_value ? v_turns : turns)[j] = make_double2(c, s);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-
-        // element d of row r's head, before anything is done to it
-        auto element = [&](int row, int column, int d, int size) { return d < size ? to_float(rows[(size_t)row * a.stride + column + d]) : 0.0f; };
-        auto norm_factor = [&](float sum) { return rsqrtf(sum / (float)a.dim + a.eps); };
-        // where the pair of element d lies, its number, and whether d is the first of the two
-        auto partner = [&](const Turn& turn, int d, int& pair, bool& is_first) {
-            const int half = turn.dims / 2;
-            pair = turn.neighbours ? d / 2 : d % half;
-            is_first = turn.neighbours ? d % 2 == 0 : d < half;
-            return turn.neighbours ? d ^ 1 : is_first ? d + half : d - half;
-        };
-
-        const int jobs = kept ? 2 * a.n_kv_heads : 0;
-        const int q_jobs = a.q_at >= 0 ? count * a.n_heads : 0;
-        for (int job = blockIdx.y * waves + wave; job < jobs + q_jobs; job += gridDim.y * waves) {
-            if (job >= jobs) {   // a row's query head
-                const int row = (job - jobs) / a.n_heads, head = (job - jobs) % a.n_heads;
-                const int column = a.q_at + head * a.dim;
-                float x[E], factor = 1.0f;
-                const bool normed = a.q_gain != nullptr || a.unit;
-#pragma unroll
-                for (int e = 0; e < E; e++) x[e] = element(first + row, column, lane + e * WAVE, a.dim);
-                if (normed) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < E; e++) sum += x[e] * x[e];
-                    factor = norm_factor(wave_total(sum));
-                }
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const int d = lane + e * WAVE;
-                    auto weighted = [&](float value, int at) { return normed ? value * factor * (a.q_gain ? a.q_gain[at] : 1.0f) : value; };
-                    float value = d < a.dim ? weighted(x[e], d) : 0.0f;
-                    if (pairs && d < a.turn.dims) {
-                        int pair;
-                        bool is_first;
-                        const int other = partner(a.turn, d, pair, is_first);
-                        const float second = weighted(element(first + row, column, other, a.dim), other);
-                        const double2 cs = turns[row * pairs + pair];
-                        const float c = (float)cs.x, s = is_first ? -(float)cs.y : (float)cs.y;
-                        value = value * c + second * s;
-                    }
-                    if (d < a.head_size) static_cast<T*>(a.q_out)[((size_t)(first + row) * a.n_heads + head) * a.head_size + d] = from_float<T>(value);
-                }
-                continue;
-            }
-            const bool of_value = job >= a.n_kv_heads;
-            const int head = of_value ? job - a.n_kv_heads : job, size = of_value ? a.vdim : a.dim;
-            const int column = of_value ? a.v_at + head * a.vdim : a.k_at + head * a.dim;
-            const Turn& turn = of_value ? a.v_turn : a.turn;
-            const int my_pairs = of_value ? v_pairs : pairs;
-            const double2* my_turns = of_value ? v_turns : turns;
-            const bool normed = !of_value && (a.k_gain != nullptr || a.unit);
-            const int lead = slot % BLOCK_TOKENS;
-            const size_t block = (((size_t)(slot >> a.page_shift) * a.n_kv_heads + head) << (a.page_shift - 4)) + ((slot & ((1 << a.page_shift) - 1)) / BLOCK_TOKENS);
-            uint8_t* const codes = (of_value ? a.v_codes : a.k_codes) + block * BLOCK_TOKENS * a.head_size;
-            float* const scale_at = (of_value ? a.v_scales : a.k_scales) + block;
-
-            float x[BLOCK_TOKENS][E];
-            float largest = 0.0f;
-#pragma unroll
-            for (int t = 0; t < BLOCK_TOKENS; t++) {
-                float factor = 1.0f;
-#pragma unroll
-                for (int e = 0; e < E; e++) x[t][e] = t < count ? element(first + t, column, lane + e * WAVE, size) : 0.0f;
-                if (normed && t < count) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < E; e++) sum += x[t][e] * x[t][e];
-                    factor = norm_factor(wave_total(sum));
-                }
-                auto weighted = [&](float value, int at) { return normed ? value * factor * (a.k_gain ? a.k_gain[at] : 1.0f) : value; };
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const int d = lane + e * WAVE;
-                    if (t < count && d < size) {
-                        float value = weighted(x[t][e], d);
-                        if (my_pairs && d < turn.dims) {
-                            int pair;
-                            bool is_first;
-                            const int other = partner(turn, d, pair, is_first);
-                            const double second = weighted(element(first + t, column, other, size), other);
-                            const double2 cs = my_turns[t * my_pairs + pair];
-                            value = sticky(fma((double)value, cs.x, second * (is_first ? -cs.y : cs.y)));
-                        }
-                        x[t][e] = value;
-                        largest = fmaxf(largest, counted_magnitude(value));
-                    }
-                }
-            }
-            largest = wave_max_total(largest);
-            const int old = lead > 0 ? scale_exponent(*scale_at) : SCALE_LOW;
-            const int exponent = max(old, needed_exponent(largest));
-            const float inverse = two_to(-exponent), factor = exponent - old < 126 ? two_to(old - exponent) : 0.0f;
-            const bool grown = lead > 0 && exponent > old;
-            if (of_value) {
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const int d = lane + e * WAVE;
-                    if (d < a.head_size) {
-                        Vec16 piece = {{0u, 0u, 0u, 0u}};
-                        Vec16* const at = reinterpret_cast<Vec16*>(codes + d * BLOCK_TOKENS);
-                        if (count < BLOCK_TOKENS) piece = *at;
-                        uint32_t fresh[4];
-                        // this run's codes from token 0 on, then moved to where they belong
-#pragma unroll
-                        for (int w = 0; w < 4; w++)
-                            fresh[w] = four_codes(ready_for_code(x[4 * w][e], inverse), ready_for_code(x[4 * w + 1][e], inverse), ready_for_code(x[4 * w + 2][e], inverse),
-                                                  ready_for_code(x[4 * w + 3][e], inverse));
-#pragma unroll
-                        for (int w = 0; w < 4; w++) {
-                            const uint32_t held = grown ? rescaled_codes(piece.w[w], factor) : piece.w[w];
-                            uint32_t out = 0;
-#pragma unroll
-                            for (int b = 0; b < 4; b++) {
-                                const int token = 4 * w + b, from = token - lead;
-                                uint32_t code = token < lead ? held >> (8 * b) : piece.w[w] >> (8 * b);
-                                if (from >= 0 && from < count) {
-                                    const uint32_t word = from < 4 ? fresh[0] : from < 8 ? fresh[1] : from < 12 ? fresh[2] : fresh[3];
-                                    code = word >> (8 * (from & 3));
-                                }
-                                out |= (code & 255u) << (8 * b);
-                            }
-                            piece.w[w] = out;
-                        }
-                        *at = piece;
-                    }
-                }
-            } else {
-                if (grown)
-                    for (int i = lane; i < a.head_size; i += WAVE)   // (head_size / 16) x 16 pieces of 16 bytes
-                        if (i % BLOCK_TOKENS < lead) {
-                            Vec16* const at = reinterpret_cast<Vec16*>(codes) + i;
-                            Vec16 piece = *at;
-#pragma unroll
-                            for (int w = 0; w < 4; w++) piece.w[w] = rescaled_codes(piece.w[w], factor);
-                            *at = piece;
-                        }
-#pragma unroll
-                for (int t = 0; t < BLOCK_TOKENS; t++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const int d = lane + e * WAVE;
-                        if (t < count && d < a.head_size)
-                            codes[((d / 16) * BLOCK_TOKENS + lead + t) * 16 + d % 16] = (uint8_t)four_codes(ready_for_code(x[t][e], inverse), 0.0f, 0.0f, 0.0f);
-                    }
-            }
-            if (lane == 0) *scale_at = two_to(exponent);
+        const int keys = run.kept ? a.n_kv_heads : 0;
+        const int queries = a.q_at < 0 ? 0 : PIECES ? a.n_heads : a.n_heads * run.count;
+        for (int job = blockIdx.y * waves + wave; job < 2 * keys + queries; job += gridDim.y * waves) {
+            if (job < keys) {
+                if constexpr (PIECES) keys_in_pieces<T, E>(a, run, job, turns, pairs, lane);
+                else keys_by_elements<T, E>(a, run, job, turns, pairs, lane);
+            } else if (job < 2 * keys) append_values<T, E>(a, run, job - keys, v_turns, v_pairs, lane);
+            else if constexpr (PIECES) queries_in_pieces<T, E>(a, run, job - 2 * keys, turns, pairs, lane);
+            else query_by_elements<T, E>(a, run, (job - 2 * keys) / a.n_heads, (job - 2 * keys) % a.n_heads, turns, pairs, lane);
         }
-        __syncthreads();
+        if (pairs + v_pairs) __syncthreads();
     }
 }
 
-// What the cache holds at slots[row]: a wave per run of rows and head; slots that name no place give zeros.
+template <typename T>
+__device__ __forceinline__ void store_two(T* to, float a, float b) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(to) = make_float2(a, b);
+    else *reinterpret_cast<bf16x2*>(to) = bf16x2{from_float<T>(a), from_float<T>(b)};
+}
+
+// What the cache holds at slots[row]: a wave per run of rows and head; slots that name no place give zeros. Keys: a lane takes the 16
+// elements of a token that lie together. Values: the tokens of two neighbouring elements, 32 bytes; heads of at most 64 elements leave half of a
+// wave, which then takes the other half of the tokens.
 template <typename T>
 __global__ __launch_bounds__(256) void scaled_rows_kernel(const uint8_t* __restrict__ k_codes, const float* __restrict__ k_scales, const uint8_t* __restrict__ v_codes,
                                                           const float* __restrict__ v_scales, const int* __restrict__ slots, long long n_slots, T* __restrict__ k_out,
@@ -250,6 +471,7 @@ __global__ __launch_bounds__(256) void scaled_rows_kernel(const uint8_t* __restr
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
     const int window = blockIdx.x * BLOCK_TOKENS, head = blockIdx.y * 4 + wave;
     if (head >= n_kv_heads) return;
+    const size_t row_size = (size_t)n_kv_heads * head_size;
     uint32_t begins = run_begins(slots, window, n_rows, n_slots, lane);
     while (begins) {
         const int at = __builtin_ctz(begins), first = window + at;
@@ -257,19 +479,48 @@ __global__ __launch_bounds__(256) void scaled_rows_kernel(const uint8_t* __restr
         begins &= begins - 1;
         const int count = min((begins ? __builtin_ctz(begins) : 32) - at, n_rows - first);
         const int slot = slots[first];
-        const bool held = slot >= 0 && slot < n_slots;
-        const size_t block = held ? (((size_t)(slot >> page_shift) * n_kv_heads + head) << (page_shift - 4)) + ((slot & ((1 << page_shift) - 1)) / BLOCK_TOKENS) : 0;
-        const float k_scale = held ? k_scales[block] : 0.0f, v_scale = held ? v_scales[block] : 0.0f;
+        T* const k_to = k_out + (size_t)first * row_size + head * head_size;
+        T* const v_to = v_out + (size_t)first * row_size + head * head_size;
+        if (slot < 0 || slot >= n_slots) {   // a run of one row
+            for (int d = lane; d < head_size; d += WAVE) k_to[d] = v_to[d] = from_float<T>(0.0f);
+            continue;
+        }
+        const int lead = slot % BLOCK_TOKENS;
+        const size_t block = (((size_t)(slot >> page_shift) * n_kv_heads + head) << (page_shift - 4)) + ((slot & ((1 << page_shift) - 1)) / BLOCK_TOKENS);
+        const float k_scale = k_scales[block], v_scale = v_scales[block];
         const uint8_t* const k = k_codes + block * BLOCK_TOKENS * head_size;
         const uint8_t* const v = v_codes + block * BLOCK_TOKENS * head_size;
-        for (int t = 0; t < count; t++) {
-            const int token = held ? slots[first + t] % BLOCK_TOKENS : 0;
-            const size_t to = ((size_t)(first + t) * n_kv_heads + head) * head_size;
-            for (int d = lane; d < head_size; d += WAVE) {
-                const float key = held ? __builtin_amdgcn_cvt_f32_fp8((int)k[((d / 16) * BLOCK_TOKENS + token) * 16 + d % 16], 0) * k_scale : 0.0f;
-                const float value = held ? __builtin_amdgcn_cvt_f32_fp8((int)v[d * BLOCK_TOKENS + token], 0) * v_scale : 0.0f;
-                k_out[to + d] = from_float<T>(key);
-                v_out[to + d] = from_float<T>(value);
+        const int token = lane % 16 - lead;
+        if (token >= 0 && token < count)
+            for (int piece = lane / 16; 16 * piece < head_size; piece += 4) {
+                const Vec16 codes = reinterpret_cast<const Vec16*>(k)[piece * BLOCK_TOKENS + lane % 16];
+                T* const to = k_to + token * row_size + 16 * piece;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float x[8];
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes.w[2 * h + w], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes.w[2 * h + w], true);
+                        x[4 * w] = lo[0] * k_scale, x[4 * w + 1] = lo[1] * k_scale, x[4 * w + 2] = hi[0] * k_scale, x[4 * w + 3] = hi[1] * k_scale;
+                    }
+                    store_eight(to + 8 * h, x);
+                }
+            }
+        const int shares = head_size <= 64 ? 2 : 1, share = shares == 2 ? lane / 32 : 0, words = 4 / shares;
+        for (int d = 2 * (shares == 2 ? lane % 32 : lane); d < head_size; d += shares == 2 ? 64 : 128) {
+            const Vec16 a = reinterpret_cast<const Vec16*>(v)[d], b = reinterpret_cast<const Vec16*>(v)[d + 1];
+            T* const to = v_to + d;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if (w / words != share) continue;
+                const f32x2 a_lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)a.w[w], false), a_hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)a.w[w], true);
+                const f32x2 b_lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.w[w], false), b_hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.w[w], true);
+                const float x[4] = {a_lo[0], a_lo[1], a_hi[0], a_hi[1]}, y[4] = {b_lo[0], b_lo[1], b_hi[0], b_hi[1]};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = 4 * w + i - lead;
+                    if (t >= 0 && t < count) store_two(to + t * row_size, x[i] * v_scale, y[i] * v_scale);
+                }
             }
         }
     }
@@ -286,12 +537,13 @@ int shift_of(int page_size) {
 MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, int k_at, int v_at, const float* q_gain, const float* k_gain, float eps, int unit,
                                 const double* frequencies, int rot_dims, int neighbours, const double* v_frequencies, int v_rot_dims, int v_neighbours,
                                 const int* positions, const int* slots, void* q_out, void* k_codes, float* k_scales, void* v_codes, float* v_scales, int num_pages,
-                                int n_rows, int n_heads, int n_kv_heads, int dim, int vdim, int head_size, int page_size, int dtype, hipStream_t stream) {
+                                int n_rows, int n_heads, int n_kv_heads, int dim, int vdim, int head_size, int page_size, int dtype, int q_dtype,
+                                hipStream_t stream) {
     MLLM_REQUIRE(n_rows >= 0 && n_heads > 0 && n_kv_heads > 0 && num_pages > 0, "scaled_append: bad sizes");
     MLLM_REQUIRE(head_size > 0 && head_size % 16 == 0 && head_size <= SCALED_MAX_HEAD && dim > 0 && dim <= head_size && vdim > 0 && vdim <= head_size,
                  "scaled_append: heads of %d and %d in pages for %d (a multiple of 16 up to %d)", dim, vdim, head_size, SCALED_MAX_HEAD);
     MLLM_REQUIRE(page_size >= BLOCK_TOKENS && (page_size & (page_size - 1)) == 0, "scaled_append: page size %d is no power of two of at least %d", page_size, BLOCK_TOKENS);
-    MLLM_REQUIRE(dtype == MLLM_F32 || dtype == MLLM_BF16, "scaled_append: unknown dtype %d", dtype);
+    MLLM_REQUIRE((dtype == MLLM_F32 || dtype == MLLM_BF16) && (q_dtype == MLLM_F32 || q_dtype == MLLM_BF16), "scaled_append: unknown dtype %d or %d", dtype, q_dtype);
     MLLM_REQUIRE(q_at >= 0 || k_at >= 0, "scaled_append: neither queries nor keys");
     MLLM_REQUIRE((k_at >= 0) == (v_at >= 0), "scaled_append: keys and values are kept together");
     MLLM_REQUIRE(rot_dims >= 0 && rot_dims % 2 == 0 && rot_dims <= dim && v_rot_dims >= 0 && v_rot_dims % 2 == 0 && v_rot_dims <= vdim, "scaled_append: the rotation does not fit the heads");
@@ -302,24 +554,31 @@ MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, in
                  "scaled_append: a missing operand");
     AppendArguments a = {rows, stride, q_at, k_at, v_at, q_gain, k_gain, eps, unit, {rot_dims ? frequencies : nullptr, rot_dims, neighbours},
                          {v_rot_dims ? v_frequencies : nullptr, v_rot_dims, v_neighbours}, positions, slots, q_out, (uint8_t*)k_codes, k_scales, (uint8_t*)v_codes, v_scales,
-                         (long long)num_pages * page_size, n_rows, n_heads, n_kv_heads, dim, vdim, head_size, shift_of(page_size)};
+                         (long long)num_pages * page_size, n_rows, n_heads, n_kv_heads, dim, vdim, head_size, shift_of(page_size), q_dtype == MLLM_F32};
+    // pieces of eight elements: everything lies on 16 bytes, and what turns with each other lies in whole pieces
+    const int size = dtype == MLLM_F32 ? 4 : 2;
+    const bool on_pieces = (uintptr_t)rows % 16 == 0 && stride * size % 16 == 0 && dim % 16 == 0 && rot_dims % 16 == 0 && (q_at < 0 || (q_at * size % 16 == 0 && (uintptr_t)q_out % 16 == 0)) &&
+                           (k_at < 0 || k_at * size % 16 == 0);
+    // many rows: 16 to a block of threads, which finds the runs among them; few: a block each, so that each is under way at once
     const int per = n_rows >= 256 && k_at >= 0 ? BLOCK_TOKENS : 1;
     const int blocks = ceil_div(n_rows, per);
-    const int jobs = (k_at >= 0 ? 2 * n_kv_heads : 0) + (q_at >= 0 ? n_heads * per : 0);
+    const int jobs = (k_at >= 0 ? 2 * n_kv_heads : 0) + (q_at < 0 ? 0 : on_pieces ? n_heads : n_heads * per);
     int shares = 1;
-    while (blocks * shares < 1024 && shares * 4 < jobs) shares *= 2;
+    while (blocks * shares < APPEND_BLOCKS && shares * 4 < jobs) shares *= 2;
     const dim3 grid(blocks, shares);
     const size_t lds = (size_t)BLOCK_TOKENS * (rot_dims / 2 + v_rot_dims / 2) * sizeof(double2);
     mllm_count_kernel(MLLM_K_SCALED_APPEND);
-#define APPEND_CASE(T, E) scaled_append_kernel<T, E><<<grid, 256, lds, stream>>>(a, per)
+#define APPEND_CASE(T, E)                                                              \
+    if (on_pieces) scaled_append_kernel<T, E, true><<<grid, 256, lds, stream>>>(a, per); \
+    else scaled_append_kernel<T, E, false><<<grid, 256, lds, stream>>>(a, per);
     if (dtype == MLLM_F32) {
-        if (head_size <= 64) APPEND_CASE(float, 1);
-        else if (head_size <= 128) APPEND_CASE(float, 2);
-        else APPEND_CASE(float, 4);
+        if (head_size <= 64) { APPEND_CASE(float, 1) }
+        else if (head_size <= 128) { APPEND_CASE(float, 2) }
+        else { APPEND_CASE(float, 4) }
     } else {
-        if (head_size <= 64) APPEND_CASE(bf16_t, 1);
-        else if (head_size <= 128) APPEND_CASE(bf16_t, 2);
-        else APPEND_CASE(bf16_t, 4);
+        if (head_size <= 64) { APPEND_CASE(bf16_t, 1) }
+        else if (head_size <= 128) { APPEND_CASE(bf16_t, 2) }
+        else { APPEND_CASE(bf16_t, 4) }
     }
 #undef APPEND_CASE
     return mllm_check_launch("scaled_append");

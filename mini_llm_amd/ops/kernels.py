@@ -1571,7 +1571,7 @@ def _rotation(frequencies, dims: int, most: int, pairing: str, name: str):
 
 def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_pages, v_pages, slots, positions, n_heads: int, n_kv_heads: int, dim: int, vdim: int, *, q_gain=None,
                   k_gain=None, unit: bool = False, eps: float = 0.0, frequencies=None, rot_dims: int = 0, pairing: str = "half", v_frequencies=None, v_rot_dims: int = 0,
-                  v_pairing: str = "half"):
+                  v_pairing: str = "half", out_dtype=None):
     """The row-wise work between a mixer's input product and its attention over pages of 8 bits (``ScaledPages``), in one kernel. ``rows``
     (float32 or bfloat16; rows may be strided): the queries [n_heads, dim] at column ``q_at`` (None: no queries are made), the keys [n_kv_heads, dim]
     at ``k_at`` and the values [n_kv_heads, vdim] at ``v_at`` (both None: the layer reads pages another layer keeps, and only its queries are
@@ -1584,7 +1584,7 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     is written begins afresh; a block that is carried on keeps its scale or, if the new rows need a larger one, is taken to that (its earlier
     tokens' codes rounded again). Tokens of a block behind those written stay as they are.
 
-    Returns the queries [rows, n_heads * head_size] in the rows' type, zeros behind their ``dim`` elements (None without ``q_at``)."""
+    Returns the queries [rows, n_heads * head_size] of ``out_dtype`` (default: the rows' type), zeros behind their ``dim`` elements (None without ``q_at``)."""
     _, _, page_size, head_size = k_pages.shape
     _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
     _require(isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _DTYPE_CODE and (rows.stride(1) == 1 or rows.shape[1] == 1),
@@ -1611,12 +1611,13 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
         _require(slots.shape[0] >= n, "fewer slots than rows")
         _require(k_pages.shape[0] * page_size <= 2**31, "the pages hold more tokens than a slot can name")
     _one_device(rows, k_pages.codes, v_pages.codes, positions, slots if keeps else None, q_gain, k_gain, frequencies, v_frequencies)
-    q = torch.empty((n, n_heads * head_size), dtype=rows.dtype, device=rows.device) if makes else None
+    out_dtype = out_dtype or rows.dtype
+    q = torch.empty((n, n_heads * head_size), dtype=out_dtype, device=rows.device) if makes else None
     check(library().mllm_scaled_append(_ptr(rows), rows.stride(0), int(q_at) if makes else -1, int(k_at) if keeps else -1, int(v_at) if keeps else -1, _ptr(q_gain), _ptr(k_gain),
                                        float(eps), int(bool(unit)), _ptr(frequencies), rot_dims, int(pairing == "neighbours"), _ptr(v_frequencies), v_rot_dims,
                                        int(v_pairing == "neighbours"), _ptr(positions), _ptr(slots if keeps else None), _ptr(q), _ptr(k_pages.codes), _ptr(k_pages.scales),
                                        _ptr(v_pages.codes), _ptr(v_pages.scales), k_pages.shape[0], n, n_heads, n_kv_heads, int(dim), int(vdim), head_size, page_size,
-                                       _code(rows.dtype), _stream()))
+                                       _code(rows.dtype), _code(out_dtype), _stream()))
     return q
 
 
