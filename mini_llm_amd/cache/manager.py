@@ -36,8 +36,9 @@ class RequestCache:
 
 class CacheManager:
     def __init__(self, groups, state_needs, *, num_pages, page_size: int, max_requests: int, dtype=None,
-                 device=None, max_length: int | None = None):
-        """groups: list of CacheGroupSpec; state_needs: {state layer: StateNeed}; num_pages: one
+                 device=None, max_length: int | None = None, scaled: bool = False):
+        """``scaled``: keys and values in 8 bits with a scale for every 16 tokens of a head (ops.kernels.ScaledPages) instead of ``dtype``.
+        groups: list of CacheGroupSpec; state_needs: {state layer: StateNeed}; num_pages: one
         number for every group or {group name: number}. ``device`` None keeps the bookkeeping only
         (tests of the manager's decisions need no GPU)."""
         if page_size < 1 or page_size & (page_size - 1):
@@ -50,7 +51,16 @@ class CacheManager:
         self.requests: dict = {}
         self._free_slots = list(range(max_requests - 1, -1, -1))
         self.state_needs = dict(state_needs)
-        self.device, self.dtype = device, dtype
+        self.device, self.dtype, self.scaled = device, dtype, bool(scaled)
+        if scaled:
+            from ..ops.kernels import SCALE_BLOCK, SCALED_MAX_HEAD
+
+            if page_size < SCALE_BLOCK:
+                raise ValueError(f"a cache of 8 bits has pages of at least {SCALE_BLOCK} tokens, not {page_size}")
+            for g in self.groups:
+                if g.head_size % 16 or not 0 < g.head_size <= SCALED_MAX_HEAD or getattr(g, "planes", 2) != 2:
+                    raise ValueError(f"a cache of 8 bits holds keys and values of heads of a multiple of 16 elements up to {SCALED_MAX_HEAD}: group {g.name} has "
+                                     f"{getattr(g, 'planes', 2)} plane(s) of {g.head_size}")
         self.k_pages, self.v_pages, self.state = {}, {}, {}
         # Per request, whatever the model: the token the sampler chose last, kept on the device so
         # that the next step can start before the host has seen it (the reference keeps such a
@@ -62,6 +72,12 @@ class CacheManager:
             self.last_token = torch.zeros((max_requests,), dtype=torch.int32, device=device)
 
             for gi, g in enumerate(self.groups):
+                if scaled:
+                    from ..ops.kernels import scaled_pages
+
+                    for layer in g.layers:
+                        self.k_pages[layer], self.v_pages[layer] = scaled_pages(self.pools[gi].num_pages, g.n_kv_heads, page_size, g.head_size, device)
+                    continue
                 planes = getattr(g, "planes", 2)
                 shape = (len(g.layers), planes, self.pools[gi].num_pages, g.n_kv_heads, page_size, g.head_size)
                 store = torch.empty(shape, dtype=dtype, device=device)
@@ -217,12 +233,16 @@ class CacheManager:
 
     def read_kv(self, request_id, layer: int, rows: int):
         """The first ``rows`` keys and values of a request in one cache layer, gathered through
-        its block table: ([rows, n_kv_heads, head_size], same). For tests and debugging (the
+        its block table: ([rows, n_kv_heads, head_size], same; float32 of a cache of 8 bits). For tests and debugging (the
         reference's gpt2_gpu_kv_cache_copy_layer, engine/src/gpt2_gpu.cu:185-195)."""
         import torch
 
         gi = self.group_of_layer[layer]
         slots = torch.tensor([self.slot(request_id, gi, p) for p in range(rows)], device=self.device)
+        if self.scaled:
+            from ..ops.kernels import scaled_rows
+
+            return scaled_rows(self.k_pages[layer], self.v_pages[layer], slots.to(torch.int32), out_dtype=torch.float32)
         pages, offsets = slots // self.page_size, slots % self.page_size
         return self.k_pages[layer][pages, :, offsets, :], self.v_pages[layer][pages, :, offsets, :]
 

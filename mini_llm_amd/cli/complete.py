@@ -21,6 +21,7 @@ def parse_args(argv=None) -> argparse.Namespace:
     parser.add_argument("--top-p", type=float, default=0.95)
     parser.add_argument("--device", default="auto", choices=("auto", "cpu", "cuda"), help="Inference device")
     parser.add_argument("--dtype", default="bfloat16", choices=("bfloat16", "float32"))
+    parser.add_argument("--cache-dtype", default=None, choices=("float8",), help="Keep keys and values in 8 bits (default: in --dtype)")
     parser.add_argument("--seed", type=int, default=0, help="Seed of the sampler")
     parser.add_argument("--max-length", type=int, default=4096, help="Longest sequence, prompt and continuation: needed for a model without a position "
                         "limit of its own (the cache holds four of them), and narrows a model's own")
@@ -54,7 +55,7 @@ def main(argv=None) -> int:
         return 2
     from ..engine.engine import Engine, EngineOptions
 
-    engine = Engine(args.model, EngineOptions(dtype=args.dtype, max_sessions=4, max_length=args.max_length))
+    engine = Engine(args.model, EngineOptions(dtype=args.dtype, max_sessions=4, max_length=args.max_length, cache_dtype=args.cache_dtype))
     tokenizer = load_tokenizer(args.model)
     eos = engine.config.eos_token_id
 

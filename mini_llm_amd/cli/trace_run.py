@@ -32,6 +32,7 @@ def main(argv=None, steps=None, out=None) -> int:
     parser.add_argument("--out", required=True, help="folder for the <step>.f32 files")
     parser.add_argument("--max-tokens", type=int, required=True, help="most tokens live requests hold at any time")
     parser.add_argument("--page-size", type=int, default=None, help="tokens per cache page (default: the engine's)")
+    parser.add_argument("--cache-dtype", default=None, choices=("float8",), help="keep keys and values in 8 bits (default: in --dtype)")
     parser.add_argument("--max-requests", type=int, default=4, help="requests that are live at any time: the cache has as many state slots")
     parser.add_argument("--hidden-out", default=None, help="folder for the residual stream after the embedding and after each layer")
     args = parser.parse_args(argv)
@@ -49,7 +50,8 @@ def main(argv=None, steps=None, out=None) -> int:
     max_tokens = args.max_tokens if page_size <= 64 else -(-args.max_tokens // 64) * page_size
     # a model without a position limit of its own: no request can hold more than the pool does
     max_length = model.max_positions() or -(-max_tokens // page_size) * page_size
-    cache = make_cache(model, max_tokens=max_tokens, page_size=page_size, max_requests=args.max_requests, device=device, max_length=max_length)
+    cache = make_cache(model, max_tokens=max_tokens, page_size=page_size, max_requests=args.max_requests, device=device, max_length=max_length,
+                       cache_dtype=args.cache_dtype)
     runner = ModelRunner(model, cache, device)
     out_dir = Path(args.out)
     out_dir.mkdir(parents=True, exist_ok=True)

@@ -15,7 +15,7 @@ import numpy as np
 
 from ..sampling import SamplingParams
 from .batch import StepEntry
-from .loading import DEFAULT_PAGE_SIZE, load_model, make_cache, random_model, tokens_for_memory
+from .loading import DEFAULT_PAGE_SIZE, load_model, make_cache, random_model, scaled_cache, tokens_for_memory
 from .scheduler import Request, Scheduler
 from .step import ModelRunner
 
@@ -29,6 +29,7 @@ class EngineOptions:
     max_sessions: int = 64
     max_tokens: int | None = None        # cache capacity in tokens; None: max_sessions full contexts
     cache_gib: float | None = None       # or the capacity as memory: GiB of page pools (an MI355X has 288 GB to give)
+    cache_dtype: str | None = None       # "float8": keys and values in 8 bits with a scale for every 16 tokens of a head (None: in ``dtype``)
     page_size: int = DEFAULT_PAGE_SIZE
     max_length: int | None = None        # longest sequence a request may reach: needed for a model without a position limit of its own, and narrows a model's own
     max_tokens_per_step: int = 2048      # token budget of one scheduler step
@@ -158,7 +159,7 @@ class Engine:
             raise ValueError("give the cache's capacity as max_tokens or as cache_gib, not both")
         if options.cache_gib is not None:
             element_size = torch.empty((), dtype=self.model.precision.compute).element_size()
-            max_tokens = tokens_for_memory(self.model.cache_groups(), element_size, options.cache_gib, options.page_size)
+            max_tokens = tokens_for_memory(self.model.cache_groups(), element_size, options.cache_gib, options.page_size, scaled_cache(self.model, options.cache_dtype))
         elif options.max_tokens is not None:
             max_tokens = options.max_tokens
         elif limit is not None:
@@ -172,7 +173,7 @@ class Engine:
             # not taken from the size of the pool (which may be millions of tokens).
             raise ValueError("this model has no position limit of its own: give max_length, the longest sequence a request may reach")
         self.cache = make_cache(self.model, max_tokens=max_tokens, page_size=options.page_size,
-                                max_requests=options.max_sessions, device=options.device, max_length=limit)
+                                max_requests=options.max_sessions, device=options.device, max_length=limit, cache_dtype=options.cache_dtype)
         self.runner = ModelRunner(self.model, self.cache, options.device, use_graphs=options.use_graphs, portion_graph_after=options.portion_graph_after,
                                   lanes_from=options.decode_lanes_from)
         self.sampler = Sampler(self.runner.staging)

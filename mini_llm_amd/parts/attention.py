@@ -26,6 +26,7 @@ MAX_HEAD_SIZE = 256
 
 class CausalSelfAttention(Mixer):
     graph_safe = True
+    takes_scaled_pages = True
     short_portion = kernels.DECODE_MAX_Q_LEN   # what the split-key kernel takes
     decode_reaches = kernels.DECODE_LAYER_REACHES
 
@@ -55,6 +56,8 @@ class CausalSelfAttention(Mixer):
     def _fused_qkv(self, ctx: LayerContext, dtype) -> bool:
         """One kernel projects, keeps q and puts keys and values into their pages."""
         page_size = ctx.k_pages.shape[2]
+        if isinstance(ctx.k_pages, kernels.ScaledPages):
+            return False
         return bool(ctx.write_cache and self.width % (16 // (4 if dtype == torch.float32 else 2)) == 0 and page_size & (page_size - 1) == 0)
 
     def forward(self, x, residual, ctx: LayerContext):
@@ -66,7 +69,11 @@ class CausalSelfAttention(Mixer):
         else:
             qkv = self.qkv.forward(x)
             q = qkv[:, : self.q_width]
-            if ctx.write_cache:
+            if isinstance(ctx.k_pages, kernels.ScaledPages):
+                if ctx.write_cache:
+                    kernels.scaled_append(qkv, None, self.q_width, self.q_width + self.kv_width, ctx.k_pages, ctx.v_pages, ctx.group.slots, ctx.batch.positions,
+                                          self.n_heads, self.n_kv_heads, self.head_size, self.head_size)
+            elif ctx.write_cache:
                 k = qkv[:, self.q_width : self.q_width + self.kv_width]
                 v = qkv[:, self.q_width + self.kv_width :]
                 kernels.cache_write(k, v, ctx.k_pages, ctx.v_pages, ctx.group.slots, self.n_kv_heads, self.head_size)

@@ -83,7 +83,7 @@ class LayerContext:
     """What the step function hands a mixer for one layer call."""
 
     batch: object                 # engine.batch.StepBatch: tokens, positions, requests
-    k_pages: object = None        # [num_pages, n_kv_heads, page_size, head_size] of the call's cache layer
+    k_pages: object = None        # [num_pages, n_kv_heads, page_size, head_size] of the call's cache layer (or ops.kernels.ScaledPages)
     v_pages: object = None
     group: object = None          # cache.GroupStepData: block tables and write slots of the layer's group
     write_cache: bool = True      # False: the layer reads a cache another layer call has written
@@ -150,8 +150,15 @@ class Mixer(Part):
     # gates, or whose feed-forward's router, read the same rows as its mixer saves a product this way.
     carries_rows = False
 
+    # True if the mixer also keeps its keys and values in 8 bits: ``ctx.k_pages`` and ``ctx.v_pages`` may then be ops.kernels.ScaledPages.
+    takes_scaled_pages = False
+
     def kv_need(self) -> KVNeed | None:
         return None
+
+    def cache_mixers(self) -> list["Mixer"]:
+        """The mixers that read and write this one's pages: itself, if it keeps keys and values (a mixer of mixers answers for those inside it)."""
+        return [self] if self.kv_need() is not None else []
 
     def state_need(self) -> StateNeed | None:
         return None

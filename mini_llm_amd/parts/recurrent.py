@@ -260,6 +260,9 @@ class ParallelMixer(Mixer):
     def kv_need(self):
         return self.left.kv_need() or self.right.kv_need()
 
+    def cache_mixers(self):
+        return self.left.cache_mixers() + self.right.cache_mixers()
+
     def _state_sizes(self):
         return [0 if need is None else need.shape[0] for need in (self.left.state_need(), self.right.state_need())]
 

@@ -39,6 +39,7 @@ class RotaryAttention(Mixer):
     graph_safe = True
     short_portion = kernels.DECODE_MAX_Q_LEN
     carries_rows = True
+    takes_scaled_pages = True
 
     def __init__(self, width: int, n_heads: int, n_kv_heads: int, dim: int, vdim: int, scale: float, *, rotary: RotaryEncoding | None = None,
                  value_rotary: RotaryEncoding | None = None, biases: bool = True, own_keys: bool = True, qk_norm: str | None = None,
@@ -144,10 +145,17 @@ class RotaryAttention(Mixer):
         v_at = self.q_width + self.k_width if self.own_keys else None
         rotary, turn = self.rotary, self._turns_back()
         turn_dims = 0 if turn is None else turn.dims
-        q = kernels.map_rows(fused, 0, k_at, v_at, self.q_norm, self.k_norm, self.eps, None if rotary is None else rotary.frequencies64(x.device),
-                             0 if rotary is None else rotary.dims, batch.positions, ctx.group.slots, ctx.k_pages, ctx.v_pages, self.n_heads,
-                             self.n_kv_heads, 1, self.dim, self.vdim, v_frequencies=turn.frequencies64(x.device) if turn_dims else None,
-                             v_rot_dims=turn_dims, v_pairing="half" if turn is None else turn.pairing, unit=self.qk_norm == "unit")
+        if isinstance(ctx.k_pages, kernels.ScaledPages):
+            q = kernels.scaled_append(fused, 0, k_at, v_at, ctx.k_pages, ctx.v_pages, ctx.group.slots, batch.positions, self.n_heads, self.n_kv_heads, self.dim, self.vdim,
+                                      q_gain=self.q_norm, k_gain=self.k_norm, unit=self.qk_norm == "unit", eps=self.eps,
+                                      frequencies=None if rotary is None else rotary.frequencies64(x.device), rot_dims=0 if rotary is None else rotary.dims,
+                                      v_frequencies=turn.frequencies64(x.device) if turn_dims else None, v_rot_dims=turn_dims,
+                                      v_pairing="half" if turn is None else turn.pairing, out_dtype=x.dtype)
+        else:
+            q = kernels.map_rows(fused, 0, k_at, v_at, self.q_norm, self.k_norm, self.eps, None if rotary is None else rotary.frequencies64(x.device),
+                                 0 if rotary is None else rotary.dims, batch.positions, ctx.group.slots, ctx.k_pages, ctx.v_pages, self.n_heads,
+                                 self.n_kv_heads, 1, self.dim, self.vdim, v_frequencies=turn.frequencies64(x.device) if turn_dims else None,
+                                 v_rot_dims=turn_dims, v_pairing="half" if turn is None else turn.pairing, unit=self.qk_norm == "unit")
         reshape = turn is not None   # the heads' sums are turned back (and leave pages wider than the values)
         need = self._need
         mixed = kernels.paged_attention(

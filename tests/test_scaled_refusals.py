@@ -69,3 +69,36 @@ def test_cuts_fit_what_the_kernel_takes(blocks, tiles, head_size, columns):
     waves, run, runs = K.scaled_cut(blocks, tiles, head_size, columns)
     assert 1 <= waves <= 16 and waves & (waves - 1) == 0 and waves * columns * (head_size + 4) * 4 <= 65536
     assert run >= 1 and run * runs >= tiles and run * (runs - 1) < tiles and 1 <= runs <= 65535
+
+
+def test_models_whose_mixers_keep_other_rows_are_refused():
+    from conftest import TINY_A, TINY_D
+    from gimozen_cases import CASES as GIMOZEN
+    from ketolix_cases import CASES as KETOLIX
+    from mini_llm_amd.config import config_from_dict
+    from mini_llm_amd.engine.loading import build_model, scaled_cache
+
+    assert scaled_cache(build_model(config_from_dict(TINY_A), "bfloat16"), "float8")
+    assert not scaled_cache(build_model(config_from_dict(TINY_A), "bfloat16"), None)
+    for config in (*GIMOZEN.values(), *KETOLIX.values()):
+        with pytest.raises(ValueError, match="8 bits"):
+            scaled_cache(build_model(config_from_dict(config), "bfloat16"), "float8")
+    with pytest.raises(ValueError, match="unknown cache type"):
+        scaled_cache(build_model(config_from_dict(TINY_A), "bfloat16"), "int4")
+
+
+@pytest.mark.parametrize("head_size,page_size,planes", [(14, 64, 2), (272, 64, 2), (16, 8, 2), (64, 64, 1)])
+def test_groups_that_a_cache_of_8_bits_does_not_hold(head_size, page_size, planes):
+    from mini_llm_amd.cache import CacheManager
+    from mini_llm_amd.models.base import CacheGroupSpec
+
+    with pytest.raises(ValueError, match="8 bits"):
+        CacheManager([CacheGroupSpec("g", (0,), 2, head_size, None, planes)], {}, num_pages=4, page_size=page_size, max_requests=2, scaled=True)
+
+
+def test_bookkeeping_of_a_cache_of_8_bits():
+    from mini_llm_amd.cache import CacheManager
+    from mini_llm_amd.models.base import CacheGroupSpec
+
+    cache = CacheManager([CacheGroupSpec("g", (0, 1), 2, 32, None)], {}, num_pages=4, page_size=16, max_requests=2, device="cpu", max_length=64, scaled=True)
+    assert cache.k_pages[0].is_keys and not cache.v_pages[1].is_keys and cache.k_pages[1].shape == (4, 2, 16, 32)
