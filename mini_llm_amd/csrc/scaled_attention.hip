@@ -45,16 +45,19 @@ struct RowView {
     __device__ __forceinline__ bool sees() const { return request >= 0 && position >= 0; }
 };
 
+// The most waves a block of rows may have: as many as have the registers they need.
+constexpr int rows_waves(int padded, int size) { return padded == 64 ? (size == 2 ? 16 : 8) : 1024 / padded; }
+
 // Rows by themselves (decoding, short portions, and whatever else comes without the shape of portions): a block per row, group of up to 16
 // heads that share a key/value head, and run of `run_tiles` tiles; its waves take the run's tiles in turn and meet in LDS. Rows of more
 // than one run leave unnormalised sums, maximum and weight per run in `parts` ([row, head, run, head_size + 2]) for the kernel below.
 // What bounds it is the cache's bytes: 2 (head_size + 0.25) a key for all heads of the group together.
-template <typename T, int HD>
-__global__ __launch_bounds__(HD == 64 ? 1024 : HD == 128 ? 512 : 256) void scaled_rows_attention_kernel(AttendArguments a, int run_tiles, int n_runs, float* __restrict__ parts) {
+template <typename T, int HD, bool WHOLE>
+__global__ __launch_bounds__(WAVE * rows_waves(HD, sizeof(T))) void scaled_rows_attention_kernel(AttendArguments a, int run_tiles, int n_runs, float* __restrict__ parts) {
     constexpr bool WIDE = sizeof(T) == 4;
-    typedef ScaledSweep<HD, 1, WIDE> Sweep;
+    typedef ScaledSweep<HD, 1, WIDE, false, WHOLE> Sweep;
     extern __shared__ float meeting[];   // [wave][column][head_size + 4]
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, waves = blockDim.x / WAVE;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
     const int row = blockIdx.x, run = blockIdx.z;
     const int head_size = a.planes.head_size, group = a.n_heads / a.planes.n_kv_heads, sets = ceil_div(group, 16);
     const int kv_head = blockIdx.y / sets, head0 = kv_head * group + (blockIdx.y % sets) * 16;
@@ -71,16 +74,14 @@ __global__ __launch_bounds__(HD == 64 ? 1024 : HD == 128 ? 512 : 256) void scale
     const bool alone = n_runs == 1 || range.count <= run_tiles;
 
     Sweep sweep;
-    sweep.init();
+    sweep.init(head_size, lane);
     const int column = lane % 16;
     sweep.template load_query<T>(0, column < columns ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride + (head0 + column) * head_size : nullptr, head_size, a.aligned, a.negative, lane);
-    const int first[1] = {view.first}, last[1] = {view.position};
-    sweep.tiles(range, begin + wave, waves, end, a.block_tables + (size_t)view.request * a.max_blocks, a.planes, kv_head, a.scale, first, last, view.first, view.position, a.keep, lane);
+    const Columns heads = {view.position, view.position, a.window, a.chunk, a.keep};
+    sweep.tiles(range, begin + wave, waves, end, a.block_tables + (size_t)view.request * a.max_blocks, a.planes, kv_head, a.scale, heads, view.first, view.position, lane);
 
     const int pitch = head_size + 4;
-    float l = sweep.l[0];
-    l += __shfl_xor(l, 16, WAVE);
-    l += __shfl_xor(l, 32, WAVE);
+    const float l = sweep.weight_sum(0);
     // the maximum is the same in the four lanes of a column: it is only raised together
     float* const mine = meeting + (wave * columns + column) * pitch;
     if (column < columns) {
@@ -147,13 +148,14 @@ __global__ __launch_bounds__(64) void scaled_merge_kernel(AttendArguments a, int
 
 // Portions of prompts: a block per (request, head, tile of 16 CT rows), whose waves hold all those rows and take the tiles of keys in turn,
 // each with statistics of its own, and meet in LDS. Tiles with the most keys come first.
-template <typename T, int HD, int CT>
-__global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void scaled_tiles_attention_kernel(AttendArguments a) {
+template <typename T, int HD, int CT, bool WHOLE>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention_kernel(AttendArguments a) {
     constexpr bool WIDE = sizeof(T) == 4;
-    typedef ScaledSweep<HD, CT, WIDE> Sweep;
+    typedef ScaledSweep<HD, CT, WIDE, true, WHOLE> Sweep;
     constexpr int ROWS = 16 * CT, WAVES = 4;
     __shared__ float meeting[WAVES / 2][CT][Sweep::DT + 1][4][WAVE];   // what half of the waves hold, lane by lane
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    __shared__ bf16x8 queries[Sweep::Q_PIECES];
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int request = blockIdx.z, head = blockIdx.y, head_size = a.planes.head_size;
     const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
     const int row0 = (gridDim.x - 1 - blockIdx.x) * ROWS;
@@ -164,25 +166,24 @@ __global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void scaled_tiles_atte
     const int position0 = min(context + row0, reach), position1 = min(context + min(row0 + ROWS, q_len) - 1, reach);
 
     Sweep sweep;
-    sweep.init();
-    int first[CT], last[CT];
+    sweep.init(head_size, lane);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
         const int local = row0 + 16 * ct + lane % 16;
         const bool valid = local < q_len;
-        last[ct] = min(context + (valid ? local : q_len - 1), reach);
-        first[ct] = scaled_first_key(last[ct], a.window, a.chunk);
-        sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
+        if (ct % WAVES == wave) {
+            sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
+            sweep.share_query(ct, queries, lane);
+        }
     }
+    sweep.q_shared = queries;
+    __syncthreads();
     const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
-    sweep.tiles(range, wave, WAVES, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale, first, last,
-                scaled_first_key(position1, a.window, a.chunk), position0, a.keep, lane);
+    sweep.tiles(range, wave, WAVES, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale,
+                {context + row0 + lane % 16, position1, a.window, a.chunk, a.keep}, scaled_first_key(position1, a.window, a.chunk), position0, lane);
 
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        sweep.l[ct] += __shfl_xor(sweep.l[ct], 16, WAVE);
-        sweep.l[ct] += __shfl_xor(sweep.l[ct], 32, WAVE);
-    }
+    for (int ct = 0; ct < CT; ct++) sweep.l[ct] = sweep.weight_sum(ct);
     // the waves' sums: the upper half's into the lower half's, then wave 1's into wave 0's
 #pragma unroll
     for (int half = WAVES / 2; half >= 1; half /= 2) {
@@ -274,7 +275,7 @@ MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const
                                          n_kv_heads, head_size, page_size, window, scale, dtype, softcap, sinks, chunk, keep, wide_out);
     a.token_request = token_request, a.positions = positions, a.out_packed = out_packed;
     if (int status = refuse_attend("scaled_attention_rows", a, page_size, dtype)) return status;
-    const int padded = head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256, most = 1024 / padded;
+    const int padded = head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256, most = rows_waves(padded, dtype == MLLM_F32 ? 4 : 2);
     MLLM_REQUIRE(waves >= 1 && waves <= most && run_tiles >= 1 && n_runs >= 1 && n_runs <= 65535 && (n_runs == 1 || parts != nullptr),
                  "scaled_attention_rows: %d waves (1..%d), runs of %d tiles, %d runs (with memory for more than one)", waves, most, run_tiles, n_runs);
     const int group = n_heads / n_kv_heads, columns = group < 16 ? group : 16;
@@ -284,16 +285,20 @@ MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const
     const dim3 grid(n_rows, n_kv_heads * ceil_div(group, 16), n_runs);
     MLLM_REQUIRE(grid.y <= 65535, "scaled_attention_rows: too many heads for one launch");
     mllm_count_kernel(MLLM_K_SCALED_ATTENTION_ROWS);
-#define ROWS_CASE(T)                                                                                                       \
-    if (padded == 64) scaled_rows_attention_kernel<T, 64><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);         \
-    else if (padded == 128) scaled_rows_attention_kernel<T, 128><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);  \
-    else scaled_rows_attention_kernel<T, 256><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);
+#define ROWS_LAUNCH(T, HD)                                                                                                         \
+    if (page_size >= TILE_KEYS) scaled_rows_attention_kernel<T, HD, true><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts); \
+    else scaled_rows_attention_kernel<T, HD, false><<<grid, waves * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);
+#define ROWS_CASE(T)                          \
+    if (padded == 64) { ROWS_LAUNCH(T, 64) }  \
+    else if (padded == 128) { ROWS_LAUNCH(T, 128) } \
+    else { ROWS_LAUNCH(T, 256) }
     if (dtype == MLLM_F32) {
         ROWS_CASE(float)
     } else {
         ROWS_CASE(bf16_t)
     }
 #undef ROWS_CASE
+#undef ROWS_LAUNCH
     if (int status = mllm_check_launch("scaled_attention_rows")) return status;
     if (n_runs == 1) return 0;
     mllm_count_kernel(MLLM_K_SCALED_ATTENTION_MERGE);
@@ -314,15 +319,20 @@ MLLM_API int mllm_scaled_attention_tiles(const void* q, long long q_stride, cons
     MLLM_REQUIRE(n_requests <= 65535 && n_heads <= 65535, "scaled_attention_tiles: too many requests or heads for one launch");
     if (n_rows == 0 || max_q_len <= 0) return 0;
     mllm_count_kernel(MLLM_K_SCALED_ATTENTION_TILES);
-#define TILES_CASE(T, HD, CT) scaled_tiles_attention_kernel<T, HD, CT><<<dim3(ceil_div(max_q_len, 16 * CT), n_heads, n_requests), 256, 0, stream>>>(a)
+#define TILES_CASE(T, HD, CT)                                                                                   \
+    {                                                                                                           \
+        const dim3 grid(ceil_div(max_q_len, 16 * CT), n_heads, n_requests);                                     \
+        if (page_size >= TILE_KEYS) scaled_tiles_attention_kernel<T, HD, CT, true><<<grid, 256, 0, stream>>>(a); \
+        else scaled_tiles_attention_kernel<T, HD, CT, false><<<grid, 256, 0, stream>>>(a);                       \
+    }
     if (dtype == MLLM_F32) {
-        if (head_size <= 64) TILES_CASE(float, 64, 2);
-        else if (head_size <= 128) TILES_CASE(float, 128, 2);
-        else TILES_CASE(float, 256, 1);
+        if (head_size <= 64) TILES_CASE(float, 64, 2)
+        else if (head_size <= 128) TILES_CASE(float, 128, 1)
+        else TILES_CASE(float, 256, 1)
     } else {
-        if (head_size <= 64) TILES_CASE(bf16_t, 64, 4);
-        else if (head_size <= 128) TILES_CASE(bf16_t, 128, 4);
-        else TILES_CASE(bf16_t, 256, 2);
+        if (head_size <= 64) TILES_CASE(bf16_t, 64, 4)
+        else if (head_size <= 128) TILES_CASE(bf16_t, 128, 2)
+        else TILES_CASE(bf16_t, 256, 1)
     }
 #undef TILES_CASE
     return mllm_check_launch("scaled_attention_tiles");

@@ -55,6 +55,12 @@ struct TileRange {
     }
 };
 
+// What the columns of a sweep see. Column r of group ct is the row at position min(position + 16 ct, most) (heads of one row: all at `most`); it
+// sees the keys from its first (scaled_first_key) up to itself, and those below `keep`.
+struct Columns {
+    int position, most, window, chunk, keep;
+};
+
 struct ScoreScale {
     float factor;       // of a raw score: |scale|, times log2 e where weights are powers of two
     float cap_in, cap;  // cap > 0: score <- cap tanh(raw cap_in), cap times log2 e where weights are powers of two
@@ -66,22 +72,38 @@ __device__ __forceinline__ float weight_of(float x) {
     else return __builtin_amdgcn_exp2f(x);
 }
 
-template <int HD, int CT, bool WIDE>
+// APART: the columns are rows at positions of their own (else heads of one row, which see the same keys). WHOLE: pages of 64 tokens or more, so a
+// tile lies in one page, which is looked up once by the scalar unit, and a lane's place in a tile is the same in every tile; smaller pages are
+// looked up by each lane for its block.
+template <int HD, int CT, bool WIDE, bool APART, bool WHOLE>
 struct ScaledSweep {
     static constexpr int NC = HD / 64, DT = HD / 16, NP = WIDE ? 3 : 1;
 
-    bf16x8 q[CT][NC][2][NP];
+    // The queries' operands: rows of a portion, which all waves of a block share, in LDS ([CT][NC][2][NP][WAVE]); a row's heads in registers.
+    bf16x8 q[APART ? 1 : CT][NC][2][NP];
+    const bf16x8* q_shared;
     f32x4 o[CT][DT];
     f32x4 s[CT][4];
+    // The running maximum and sum. In bfloat16 the weights are summed by the matrix instructions, as another row of values that are all 1 (what is
+    // summed is what the values are weighted with), and every lane of a column has the whole sum; in 32-bit a lane has its own keys'.
     float m[CT], l[CT];
+    f32x4 l_rows[WIDE ? 1 : CT];
     Vec16 k_raw[4][NC], v_raw[DT];
     float k_scale, v_scale;
+    int k_lane[NC], v_lane, head_size;   // where a lane's pieces lie, in bytes
 
-    __device__ __forceinline__ void init() {
+    __device__ __forceinline__ void init(int head_size_, int lane) {
+        head_size = head_size_;
+        const int quarter = lane / 16, r = lane % 16, block = BLOCK_TOKENS * head_size;
+#pragma unroll
+        for (int c = 0; c < NC; c++)   // (pieces beyond the head's: its last once more, which meet zeros of the query)
+            k_lane[c] = min(4 * c + quarter, head_size / 16 - 1) * 256 + (r % 4) * 16 + (WHOLE ? r / 4 * block : 0);
+        v_lane = r * 16 + (WHOLE ? quarter * block : 0);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             m[ct] = NO_SCORE;
             l[ct] = 0.0f;
+            if constexpr (!WIDE) l_rows[ct] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
@@ -100,6 +122,7 @@ struct ScaledSweep {
     }
 
     // Column ct's query: `row` points at its head's first element (null: no query here). negative: a negative score scale, whose sign the queries take.
+    static constexpr int Q_PIECES = CT * NC * 2 * NP * WAVE;   // of 16 bytes, in LDS
     template <typename T>
     __device__ __forceinline__ void load_query(int ct, const T* row, int head_size, bool aligned, bool negative, int lane) {
         const int quarter = lane / 16;
@@ -126,70 +149,86 @@ struct ScaledSweep {
                     bf16_t piece[NP];
                     in_pieces(negative ? -to_float(x[i]) : to_float(x[i]), piece);
 #pragma unroll
-                    for (int p = 0; p < NP; p++) q[ct][c][h][p][i] = piece[p];
+                    for (int p = 0; p < NP; p++) q[APART ? 0 : ct][c][h][p][i] = piece[p];
                 }
             }
     }
+    __device__ __forceinline__ void share_query(int ct, bf16x8* to, int lane) {
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int p = 0; p < NP; p++) to[(((ct * NC + c) * 2 + h) * NP + p) * WAVE + lane] = q[0][c][h][p];
+    }
 
-    // Where the lane's block of keys (r / 4) and of values (q) of a tile lie, as numbers of blocks.
+    // Where a tile's blocks lie, as numbers of blocks: its first (WHOLE), or the lane's block of keys (r / 4) and of values (q).
     struct Places {
         long long k, v;
     };
     static __device__ __forceinline__ long long place(int block, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head) {
         const int shift = planes.page_shift - 4;
-        const unsigned page = min((unsigned)table[block >> shift], (unsigned)planes.num_pages - 1u);   // (nothing a table holds leads out of the pages)
+        unsigned page = (unsigned)table[block >> shift];
+        if constexpr (WHOLE) page = __builtin_amdgcn_readfirstlane(page);
+        page = min(page, (unsigned)planes.num_pages - 1u);   // (nothing a table holds leads out of the pages)
         return (((long long)page * planes.n_kv_heads + kv_head) << shift) + (block & ((1 << shift) - 1));
     }
     static __device__ __forceinline__ Places look_up(const TileRange& range, int tile, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head, int lane) {
         const int block = range.first_key_of(tile) / BLOCK_TOKENS;
-        return {place(range.stored(block + (lane % 16) / 4), table, planes, kv_head), place(range.stored(block + lane / 16), table, planes, kv_head)};
+        if constexpr (WHOLE) {   // (the page holds a key that is seen; what else lies in it is masked)
+            const long long at = place(block, table, planes, kv_head);
+            return {at, at};
+        } else return {place(range.stored(block + (lane % 16) / 4), table, planes, kv_head), place(range.stored(block + lane / 16), table, planes, kv_head)};
     }
 
     __device__ __forceinline__ void load_keys(const Places& at, const ScaledPlanes& planes, int lane) {
-        const int quarter = lane / 16, r = lane % 16, pieces = planes.head_size / 16;
-        const Vec16* const block = reinterpret_cast<const Vec16*>(planes.k_codes) + at.k * planes.head_size;
+        const uint8_t* const block = planes.k_codes + at.k * (BLOCK_TOKENS * head_size);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int c = 0; c < NC; c++)   // (pieces beyond the head's: its last once more, which meet zeros of the query)
-                k_raw[t][c] = block[min(4 * c + quarter, pieces - 1) * 16 + 4 * t + r % 4];
-        k_scale = planes.k_scales[at.k];
+            for (int c = 0; c < NC; c++) k_raw[t][c] = *reinterpret_cast<const Vec16*>(block + (unsigned)k_lane[c] + 64 * t);
+        k_scale = planes.k_scales[at.k + (WHOLE ? (lane % 16) / 4 : 0)];
     }
     __device__ __forceinline__ void load_values(const Places& at, const ScaledPlanes& planes, int lane) {
-        const Vec16* const block = reinterpret_cast<const Vec16*>(planes.v_codes) + at.v * planes.head_size;
-        const int tiles = planes.head_size / 16;
+        const uint8_t* const block = planes.v_codes + at.v * (BLOCK_TOKENS * head_size);
+        const int tiles = head_size / 16;
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) v_raw[dt] = block[min(dt, tiles - 1) * 16 + lane % 16];
-        v_scale = planes.v_scales[at.v];
+        for (int dt = 0; dt < DT; dt++) v_raw[dt] = *reinterpret_cast<const Vec16*>(block + (unsigned)v_lane + 256 * min(dt, tiles - 1));
+        v_scale = planes.v_scales[at.v + (WHOLE ? lane / 16 : 0)];
     }
 
-    __device__ __forceinline__ void scores() {
+    __device__ __forceinline__ void scores(int lane) {
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
 #pragma unroll
             for (int t = 0; t < 4; t++) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-            for (int c = 0; c < NC; c++)
+            for (int h = 0; h < 2; h++) {
+                bf16x8 keys[4];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const bf16x8 keys = eight_numbers(k_raw[t][c].w[2 * h], k_raw[t][c].w[2 * h + 1], k_scale);
+                for (int t = 0; t < 4; t++) keys[t] = eight_numbers(k_raw[t][c].w[2 * h], k_raw[t][c].w[2 * h + 1], k_scale);
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
+                for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                        for (int p = NP - 1; p >= 0; p--) s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys, q[ct][c][h][p], s[ct][t], 0, 0, 0);
-                }
+                    for (int p = NP - 1; p >= 0; p--) {
+                        const bf16x8 query = APART ? q_shared[(((ct * NC + c) * 2 + h) * NP + p) * WAVE + lane] : q[ct][c][h][p];
+#pragma unroll
+                        for (int t = 0; t < 4; t++) s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[t], query, s[ct][t], 0, 0, 0);
+                    }
+                if constexpr (APART) __builtin_amdgcn_sched_barrier(0);   // (operands of all the products at once would not fit the registers)
+            }
     }
 
-    // Takes the tile's scores and values into the running sums. first_key: of the tile. MASKED: some column does not see some key; a key counts
-    // for column ct if it is at most last[ct] and (at least first[ct] or below keep).
+    // Takes the tile's scores and values into the running sums. first_key: of the tile. MASKED: some column does not see some key.
     template <bool MASKED>
-    __device__ __forceinline__ void take(const ScoreScale& scale, int first_key, const int (&first)[CT], const int (&last)[CT], int keep, int lane) {
+    __device__ __forceinline__ void take(const ScoreScale& scale, int first_key, const Columns& columns, int lane) {
         const int key = first_key + BLOCK_TOKENS * (lane / 16);   // the lane's keys: key + 4 t + i
         uint32_t seen[CT];
         bool raise = false;
         float top[CT];
+        const float factor = scale.cap > 0.0f ? 1.0f : scale.factor;   // (capped scores are in their units already)
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             if (scale.cap > 0.0f) {
@@ -203,12 +242,13 @@ struct ScaledSweep {
             }
             if constexpr (MASKED) {
                 seen[ct] = 0;
+                const int last = min(columns.position + 16 * ct, columns.most), first = scaled_first_key(last, columns.window, columns.chunk);
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int k = key + 4 * t + i;
-                        const bool counts = k <= last[ct] && (k >= first[ct] || k < keep);
+                        const bool counts = k <= last && (k >= first || k < columns.keep);
                         seen[ct] |= counts ? 1u << (4 * t + i) : 0u;
                         s[ct][t][i] = counts ? s[ct][t][i] : -INFINITY;
                     }
@@ -218,7 +258,7 @@ struct ScaledSweep {
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) best = fmaxf(best, s[ct][t][i]);
-            top[ct] = scale.cap > 0.0f ? best : best * scale.factor;
+            top[ct] = best * factor;
             raise |= top[ct] > m[ct] + SCORE_SLACK;
         }
         if (__any(raise)) {
@@ -230,7 +270,10 @@ struct ScaledSweep {
                 const float higher = fmaxf(m[ct], best);
                 const float fall = weight_of<WIDE>(m[ct] - higher);
                 m[ct] = higher;
-                l[ct] *= fall;
+                if constexpr (WIDE) l[ct] *= fall;
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; i++) l_rows[ct][i] *= fall;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -245,48 +288,70 @@ struct ScaledSweep {
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float x = scale.cap > 0.0f ? s[ct][t][i] - m[ct] : WIDE ? s[ct][t][i] * scale.factor - m[ct] : __builtin_fmaf(s[ct][t][i], scale.factor, -m[ct]);
-                    const float p = weight_of<WIDE>(x);
-                    sum += p;
+                    const float p = weight_of<WIDE>(__builtin_fmaf(s[ct][t][i], factor, -m[ct]));
+                    if constexpr (WIDE) sum += p;
                     bf16_t piece[NP];
                     in_pieces(p, piece);
 #pragma unroll
                     for (int n = 0; n < NP; n++) weights[ct][t / 2][n][4 * (t % 2) + i] = piece[n];
                 }
-            l[ct] += sum;
+            if constexpr (WIDE) l[ct] += sum;
+        }
+        if constexpr (!WIDE) {
+            const bf16_t one = static_cast<bf16_t>(1.0f);
+            const bf16x8 ones = {one, one, one, one, one, one, one, one};
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) l_rows[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, weights[ct][h][0], l_rows[ct], 0, 0, 0);
         }
         if constexpr (MASKED) {
-            // Not even a weight of zero silences a NaN: where the tile has any (in places that nothing was written to, or that some column does not
-            // see), they are taken out, and each goes to the columns that see it.
+            // Not even a weight of zero silences a NaN: codes that are no number are taken out where no column sees them (places that nothing was
+            // written to, pages that others hold) ..
+            uint32_t all = 0;
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) all |= seen[ct];
+            if constexpr (APART) {
+                all |= __shfl_xor(all, 1, WAVE);
+                all |= __shfl_xor(all, 2, WAVE);
+                all |= __shfl_xor(all, 4, WAVE);
+                all |= __shfl_xor(all, 8, WAVE);
+            }
             uint32_t none = 0;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) none |= not_numbers(v_raw[dt].w[0]) | not_numbers(v_raw[dt].w[1]) | not_numbers(v_raw[dt].w[2]) | not_numbers(v_raw[dt].w[3]);
-            if (__any(none != 0)) {
+            for (int w = 0; w < 4; w++) {
+                const uint32_t bits = all >> (4 * w);   // four tokens, a byte each
+                const uint32_t bytes = ((bits & 1u) | (bits & 2u) << 7 | (bits & 4u) << 14 | (bits & 8u) << 21) * 0xffu;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) {
+                    v_raw[dt].w[w] &= bytes;
+                    if constexpr (APART) none |= not_numbers(v_raw[dt].w[w]);
+                }
+            }
+            // .. and where some do and some do not, each goes to the columns that see it.
+            if (APART && __any(none != 0)) {
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) {
                     Vec16 ones;
-                    uint32_t some = 0;
 #pragma unroll
                     for (int w = 0; w < 4; w++) {
                         const uint32_t high = not_numbers(v_raw[dt].w[w]) >> 7;   // 1 in each byte that is no number
-                        some |= high;
                         ones.w[w] = high * 0x38u;                                 // the code of 1
                         v_raw[dt].w[w] &= ~(high * 0xffu);
                     }
-                    if (__any(some != 0)) {
 #pragma unroll
-                        for (int ct = 0; ct < CT; ct++) {
-                            f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int ct = 0; ct < CT; ct++) {
+                        f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                bf16x8 sees;
+                        for (int h = 0; h < 2; h++) {
+                            bf16x8 sees;
 #pragma unroll
-                                for (int i = 0; i < 8; i++) sees[i] = static_cast<bf16_t>((seen[ct] >> (8 * h + i)) & 1u ? 1.0f : 0.0f);
-                                count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_numbers(ones.w[2 * h], ones.w[2 * h + 1], 1.0f), sees, count, 0, 0, 0);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[ct][dt][i] = count[i] > 0.0f ? __builtin_nanf("") : o[ct][dt][i];
+                            for (int i = 0; i < 8; i++) sees[i] = static_cast<bf16_t>((seen[ct] >> (8 * h + i)) & 1u ? 1.0f : 0.0f);
+                            count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_numbers(ones.w[2 * h], ones.w[2 * h + 1], 1.0f), sees, count, 0, 0, 0);
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[ct][dt][i] = count[i] > 0.0f ? __builtin_nanf("") : o[ct][dt][i];
+                        __builtin_amdgcn_sched_barrier(0);   // (a rare path: not at the price of registers)
                     }
                 }
             }
@@ -300,25 +365,52 @@ struct ScaledSweep {
                 for (int ct = 0; ct < CT; ct++)
 #pragma unroll
                     for (int n = NP - 1; n >= 0; n--) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, weights[ct][h][n], o[ct][dt], 0, 0, 0);
+                if constexpr (APART) __builtin_amdgcn_sched_barrier(0);
             }
     }
 
-    // Tiles tile, tile + step, .. below `end`. all_from / all_to: every column sees the keys all_from .. all_to (beside kept ones).
+    // Tiles tile, tile + step, .. below `end`, those that all columns see whole first, then the others (the order makes no difference): all_from /
+    // all_to: every column sees the keys all_from .. all_to (beside kept ones).
     __device__ __forceinline__ void tiles(const TileRange& range, int tile, int step, int end, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head,
-                                          const ScoreScale& scale, const int (&first)[CT], const int (&last)[CT], int all_from, int all_to, int keep, int lane) {
+                                          const ScoreScale& scale, const Columns& columns, int all_from, int all_to, int lane) {
+        // tiles whole_from .. whole_to - 1 are seen whole
+        const int whole_from = max(range.kept_tiles, range.kept_tiles + ceil_div(all_from, TILE_KEYS) - range.first_tile);
+        const int whole_to = min(end, range.kept_tiles + (all_to + 1) / TILE_KEYS - range.first_tile);
+        const int skipped = whole_from > tile ? ceil_div(whole_from - tile, step) : 0;
+        const int begin = tile + skipped * step;   // the wave's first tile that may be whole
+        const int behind = begin < whole_to ? begin + ceil_div(whole_to - begin, step) * step : begin;
+        some_tiles<false>(range, begin, step, whole_to, behind, behind, table, planes, kv_head, scale, columns, lane);
+        some_tiles<true>(range, tile < begin ? tile : behind, step, end, begin, behind, table, planes, kv_head, scale, columns, lane);
+    }
+
+    // Tiles tile, tile + step, .. below `end`, but for those of from .. to - 1.
+    template <bool MASKED>
+    __device__ __forceinline__ void some_tiles(const TileRange& range, int tile, int step, int end, int from, int to, const int* __restrict__ table, const ScaledPlanes& planes, int kv_head,
+                                               const ScoreScale& scale, const Columns& columns, int lane) {
         if (tile >= end) return;
         Places at = look_up(range, tile, table, planes, kv_head, lane);
         load_keys(at, planes, lane);
         load_values(at, planes, lane);
-        for (; tile < end; tile += step) {
-            const bool more = tile + step < end;
-            if (more) at = look_up(range, tile + step, table, planes, kv_head, lane);
-            scores();
+        while (tile < end) {
+            const int ahead = tile + step, next = ahead >= from && ahead < to ? to : ahead;
+            const bool more = next < end;
+            if (more) at = look_up(range, next, table, planes, kv_head, lane);
+            scores(lane);
             if (more) load_keys(at, planes, lane);   // the next tile's, while this one's weights are made
-            const int first_key = range.first_key_of(tile);
-            if (first_key >= all_from && first_key + TILE_KEYS - 1 <= all_to) take<false>(scale, first_key, first, last, keep, lane);
-            else take<true>(scale, first_key, first, last, keep, lane);
+            take<MASKED>(scale, range.first_key_of(tile), columns, lane);
             if (more) load_values(at, planes, lane);
+            tile = next;
+        }
+    }
+
+    // The wave's sum of weights of column ct, in every lane of it.
+    __device__ __forceinline__ float weight_sum(int ct) const {
+        if constexpr (!WIDE) return l_rows[ct][0];
+        else {
+            float sum = l[ct];
+            sum += __shfl_xor(sum, 16, WAVE);
+            sum += __shfl_xor(sum, 32, WAVE);
+            return sum;
         }
     }
 };

@@ -1639,10 +1639,10 @@ SCALED_TILE = 64            # keys a wave takes at a time
 SCALED_SHORT = 8            # portions up to so many tokens go row by row
 
 
-def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int) -> tuple[int, int, int]:
+def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int, wide: bool = False) -> tuple[int, int, int]:
     """(waves a block, tiles a run, runs) for the rows kernel over pages of 8 bits: ``blocks`` (row, head group) pairs, each with up to ``tiles`` tiles of
-    keys, ``columns`` heads of ``head_size`` a block."""
-    most = 1024 // (64 if head_size <= 64 else 128 if head_size <= 128 else 256)
+    keys, ``columns`` heads of ``head_size`` a block; ``wide``: queries in 32-bit."""
+    most = (8 if wide else 16) if head_size <= 64 else 8 if head_size <= 128 else 4
     while most > 1 and most * columns * (head_size + 4) * 4 > 65536:
         most //= 2
     run = tiles
@@ -1695,7 +1695,7 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
         tiles = -(-span // SCALED_TILE) + (2 if window or chunk else 0)
         sets = -(-(n_heads // n_kv_heads) // 16)
         longest = tiles if max_len is None else max(1, min(tiles, -(-int(max_len) // SCALED_TILE)))
-        waves, run, runs = scaled_cut(count * n_kv_heads * sets, longest, head_size, min(16, n_heads // n_kv_heads))
+        waves, run, runs = scaled_cut(count * n_kv_heads * sets, longest, head_size, min(16, n_heads // n_kv_heads), q.dtype == torch.float32)
         parts = torch.empty((count, n_heads, runs, head_size + 2), dtype=torch.float32, device=q.device) if runs > 1 else None
         check(lib.mllm_scaled_attention_rows(_ptr(q), q.stride(0), *pages, _ptr(into), width if packed else into.stride(0), _ptr(token_request), _ptr(positions),
                                              _ptr(block_tables), block_tables.shape[1], block_tables.shape[0], num_pages, count, n_heads, n_kv_heads, head_size, page_size, window,

@@ -67,6 +67,7 @@ def test_planes_in_the_wrong_place_are_refused():
 @pytest.mark.parametrize("head_size,columns", [(16, 1), (64, 16), (128, 4), (128, 16), (256, 1), (256, 16)])
 def test_cuts_fit_what_the_kernel_takes(blocks, tiles, head_size, columns):
     waves, run, runs = K.scaled_cut(blocks, tiles, head_size, columns)
+    assert K.scaled_cut(blocks, tiles, head_size, columns, True)[0] <= (8 if head_size <= 128 else 4)
     assert 1 <= waves <= 16 and waves & (waves - 1) == 0 and waves * columns * (head_size + 4) * 4 <= 65536
     assert run >= 1 and run * runs >= tiles and run * (runs - 1) < tiles and 1 <= runs <= 65535
 
