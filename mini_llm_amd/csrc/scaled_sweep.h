@@ -202,23 +202,53 @@ struct ScaledSweep {
         for (int ct = 0; ct < CT; ct++)
 #pragma unroll
             for (int t = 0; t < 4; t++) s[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        // the operands of a step are converted while the matrix cores work on the step before (two conversions fit behind a product)
+        constexpr int STEPS = 2 * NC;
+        bf16x8 keys[2][4];
+        auto convert = [&](int step) {
 #pragma unroll
-        for (int c = 0; c < NC; c++)
+            for (int t = 0; t < 4; t++) keys[step % 2][t] = eight_numbers(k_raw[t][step / 2].w[2 * (step % 2)], k_raw[t][step / 2].w[2 * (step % 2) + 1], k_scale);
+        };
+        // .. and a query's operand is on its way from LDS for the time of two
+        constexpr int AHEAD = 2, QUERIES = STEPS * CT * NP;   // number (step, ct, NP - 1 - p)
+        bf16x8 ring[AHEAD + 1];
+        auto query_at = [&](int n) {
+            const int step = n / (CT * NP), ct = n / NP % CT, p = NP - 1 - n % NP;
+            return APART ? q_shared[((ct * STEPS + step) * NP + p) * WAVE + lane] : q[APART ? 0 : ct][step / 2][step % 2][p];
+        };
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                bf16x8 keys[4];
+        for (int n = 0; n < AHEAD && n < QUERIES; n++) ring[n] = query_at(n);
+        convert(0);
 #pragma unroll
-                for (int t = 0; t < 4; t++) keys[t] = eight_numbers(k_raw[t][c].w[2 * h], k_raw[t][c].w[2 * h + 1], k_scale);
+        for (int step = 0; step < STEPS; step++) {
+            if (step + 1 < STEPS) convert(step + 1);
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++)
+            for (int i = 0; i < CT * NP; i++) {
+                const int n = step * CT * NP + i, ct = i / NP;
+                if (n + AHEAD < QUERIES) ring[(n + AHEAD) % (AHEAD + 1)] = query_at(n + AHEAD);
 #pragma unroll
-                    for (int p = NP - 1; p >= 0; p--) {
-                        const bf16x8 query = APART ? q_shared[(((ct * NC + c) * 2 + h) * NP + p) * WAVE + lane] : q[ct][c][h][p];
-#pragma unroll
-                        for (int t = 0; t < 4; t++) s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[t], query, s[ct][t], 0, 0, 0);
-                    }
-                if constexpr (APART) __builtin_amdgcn_sched_barrier(0);   // (operands of all the products at once would not fit the registers)
+                for (int t = 0; t < 4; t++) s[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(keys[step % 2][t], ring[n % (AHEAD + 1)], s[ct][t], 0, 0, 0);
             }
+            if constexpr (APART) {
+                interleave<CT * NP, 4, 16>();
+                __builtin_amdgcn_sched_barrier(0);   // (operands of all the products at once would not fit the registers)
+            }
+        }
+    }
+
+    // Asks the compiler for GROUPS of a read from LDS and PRODUCTS matrix instructions, with CONVERSIONS others spread among all of them.
+    template <int GROUPS, int PRODUCTS, int CONVERSIONS>
+    static __device__ __forceinline__ void interleave() {
+        constexpr int EACH = (CONVERSIONS + GROUPS * PRODUCTS - 1) / (GROUPS * PRODUCTS);
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++) {
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);    // a read from LDS
+#pragma unroll
+            for (int i = 0; i < PRODUCTS; i++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);    // a matrix instruction
+                __builtin_amdgcn_sched_group_barrier(0x002, EACH, 0); // others
+            }
+        }
     }
 
     // Takes the tile's scores and values into the running sums. first_key: of the tile. MASKED: some column does not see some key.
@@ -356,17 +386,22 @@ struct ScaledSweep {
                 }
             }
         }
+        bf16x8 values[2];
+        auto convert = [&](int step) { values[step % 2] = eight_numbers(v_raw[step / 2].w[2 * (step % 2)], v_raw[step / 2].w[2 * (step % 2) + 1], v_scale); };
+        convert(0);
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
+        for (int step = 0; step < 2 * DT; step++) {
+            if (step + 1 < 2 * DT) convert(step + 1);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const bf16x8 values = eight_numbers(v_raw[dt].w[2 * h], v_raw[dt].w[2 * h + 1], v_scale);
+            for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int n = NP - 1; n >= 0; n--) o[ct][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values, weights[ct][h][n], o[ct][dt], 0, 0, 0);
-                if constexpr (APART) __builtin_amdgcn_sched_barrier(0);
+                for (int n = NP - 1; n >= 0; n--)
+                    o[ct][step / 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values[step % 2], weights[ct][step % 2][n], o[ct][step / 2], 0, 0, 0);
+            if constexpr (APART) {
+                interleave<1, CT * NP, 4>();
+                if (step % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
+        }
     }
 
     // Tiles tile, tile + step, .. below `end`, those that all columns see whole first, then the others (the order makes no difference): all_from /

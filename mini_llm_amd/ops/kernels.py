@@ -1477,7 +1477,6 @@ SCALED_MAX_HEAD = 256
 E4M3 = torch.float8_e4m3fn
 
 
-@dataclass(frozen=True)
 class ScaledPages:
     """The pages of one cache layer's keys, or of its values, in 8 bits with a scale for every block of SCALE_BLOCK tokens of a head: a number
     x is held as the code nearest to x / scale, scale the smallest power of two (2^-110 .. 2^118) with 448 scale at least the block's largest
@@ -1486,41 +1485,27 @@ class ScaledPages:
     ``codes`` (float8_e4m3fn): keys [num_pages, n_kv_heads, page_size / 16, head_size / 16, 16 tokens, 16 elements], values [num_pages,
     n_kv_heads, page_size / 16, head_size, 16 tokens]: a block lies as the matrix instructions take it (csrc/scaled_blocks.h). ``scales``:
     float32 [num_pages, n_kv_heads, page_size / 16]. ``scaled_append`` writes them, ``paged_attention`` reads them where it is given them as
-    pages, ``scaled_rows`` gives what they hold. ``shape`` and ``dtype`` are as pages of plain rows have them."""
+    pages, ``scaled_rows`` gives what they hold. ``shape`` ([num_pages, n_kv_heads, page_size, head_size]) and ``dtype`` are as pages of plain
+    rows have them."""
 
-    codes: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("codes", "scales", "shape", "is_keys", "on_gpu", "device_index", "addresses")
+    dtype = E4M3
 
-    def __post_init__(self):
-        codes, scales = self.codes, self.scales
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         _require(isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor), "codes and scales are tensors")
-        _require(codes.dtype == E4M3 and scales.dtype == torch.float32, f"codes are {E4M3} and scales float32, not {codes.dtype} and {scales.dtype}")
-        _require(codes.is_contiguous() and scales.is_contiguous() and codes.device == scales.device, "codes and scales are contiguous and lie on one device")
-        _require(codes.dim() in (5, 6) and codes.shape[-1] == SCALE_BLOCK and (codes.dim() == 5 or codes.shape[-2] == SCALE_BLOCK), "codes have neither the shape of keys nor that of values")
-        _require(scales.dim() == 3 and tuple(scales.shape) == tuple(codes.shape[:3]), "one scale a block")
-        page_size, head_size = self.page_size, self.head_size
-        _require(page_size >= SCALE_BLOCK and page_size & (page_size - 1) == 0, f"page size {page_size} is no power of two of at least {SCALE_BLOCK}")
-        _require(codes.shape[0] > 0 and codes.shape[1] > 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD, f"heads of {head_size} are not a multiple of 16 up to {SCALED_MAX_HEAD}")
-
-    @property
-    def is_keys(self) -> bool:
-        return self.codes.dim() == 6
-
-    @property
-    def page_size(self) -> int:
-        return self.codes.shape[2] * SCALE_BLOCK
-
-    @property
-    def head_size(self) -> int:
-        return self.codes.shape[3] * (16 if self.is_keys else 1)
-
-    @property
-    def shape(self) -> tuple:
-        return (self.codes.shape[0], self.codes.shape[1], self.page_size, self.head_size)
-
-    @property
-    def dtype(self):
-        return self.codes.dtype
+        if codes.dtype != E4M3 or scales.dtype != torch.float32:
+            raise OperandError(f"codes are {E4M3} and scales float32, not {codes.dtype} and {scales.dtype}")
+        self.device_index = codes.get_device()   # -1: not on a GPU
+        _require(codes.is_contiguous() and scales.is_contiguous() and scales.get_device() == self.device_index, "codes and scales are contiguous and lie on one device")
+        of_codes, of_scales = tuple(codes.shape), tuple(scales.shape)
+        self.is_keys = len(of_codes) == 6
+        _require(len(of_codes) in (5, 6) and of_codes[-1] == SCALE_BLOCK and of_codes[4] == SCALE_BLOCK, "codes have neither the shape of keys nor that of values")
+        _require(of_scales == of_codes[:3], "one scale a block")
+        page_size, head_size = of_codes[2] * SCALE_BLOCK, of_codes[3] * (16 if self.is_keys else 1)
+        if not (of_codes[0] > 0 and of_codes[1] > 0 and page_size >= SCALE_BLOCK and page_size & (page_size - 1) == 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD):
+            raise OperandError(f"pages of {page_size} tokens (a power of two of at least {SCALE_BLOCK}) for heads of {head_size} (a multiple of 16 up to {SCALED_MAX_HEAD})")
+        self.codes, self.scales, self.on_gpu = codes, scales, self.device_index >= 0 and codes.is_cuda
+        self.shape, self.addresses = (of_codes[0], of_codes[1], page_size, head_size), (codes.data_ptr(), scales.data_ptr())
 
     @property
     def device(self):
@@ -1540,33 +1525,52 @@ def scaled_pages(num_pages: int, n_kv_heads: int, page_size: int, head_size: int
 def _check_scaled(k_pages, v_pages, n_kv_heads: int, head_size: int):
     if not (isinstance(k_pages, ScaledPages) and isinstance(v_pages, ScaledPages) and k_pages.is_keys and not v_pages.is_keys):
         raise OperandError("key pages and value pages of 8 bits go together, each in its place")
-    _require(k_pages.shape == v_pages.shape, "key and value pages differ in shape")
-    _require(k_pages.shape[1] == n_kv_heads and k_pages.shape[3] == head_size, "pages do not match the heads")
-    _require(k_pages.codes.is_cuda and v_pages.codes.is_cuda, "the pages are not on the GPU: there is no CPU path")
+    shape = k_pages.shape
+    _require(shape == v_pages.shape, "key and value pages differ in shape")
+    _require(shape[1] == n_kv_heads and shape[3] == head_size, "pages do not match the heads")
+    _require(k_pages.on_gpu and v_pages.on_gpu, "the pages are not on the GPU: there is no CPU path")
+    here = torch.cuda.current_device()   # kernels run on the current device's stream: what they are given lies there
+    if k_pages.device_index != here or v_pages.device_index != here:
+        raise OperandError(f"pages on cuda:{k_pages.device_index} and cuda:{v_pages.device_index} meet a kernel on the current device, cuda:{here}")
+    return here
 
 
-def _one_device(*tensors) -> None:
-    """Kernels run on the current device's stream: what they are given lies there."""
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.device.index != here:
-            raise OperandError(f"a tensor on {t.device} meets a kernel on the current device, cuda:{here}")
+def _ints(t, name: str, least: int, here: int) -> int:
+    """The address of at least so many int32 numbers in a row on the current device."""
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 1 and t.get_device() == here and t.is_contiguous() and t.numel() >= least):
+        _device_tensor(t, name, torch.int32, 1)
+        _require(t.numel() >= least, f"fewer {name} than there should be ({least})")
+        raise OperandError(f"{name} on cuda:{t.get_device()} meet a kernel on the current device, cuda:{here}")
+    return t.data_ptr()
 
 
-def _strided_rows(t, name: str, width: int) -> None:
+def _floats(t, name: str, count: int, here: int):
+    """The address of ``count`` float32 numbers on the current device (None: none)."""
+    if t is None:
+        return None
+    _device_tensor(t, name, torch.float32, 1)
+    _require(t.shape[0] == count, f"{name} does not match the heads")
+    _require(t.get_device() == here, f"{name} lies on another device than the current one")
+    return t.data_ptr()
+
+
+def _strided_rows(t, name: str, width: int, here: int) -> None:
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.shape[1] == width and (t.stride(1) == 1 or width == 1)):
         raise OperandError(f"{name} must be 2-D on the GPU with {width} contiguous columns")
     _require(t.stride(0) >= width or t.shape[0] <= 1, f"{name}'s rows overlap")
+    _require(t.get_device() == here, f"{name} lies on another device than the current one")
 
 
-def _rotation(frequencies, dims: int, most: int, pairing: str, name: str):
-    dims = int(dims or 0)
+def _rotation(frequencies, dims: int, most: int, pairing: str, name: str, here: int):
+    """(address, turned elements) of a rotation, (None, 0) of none."""
     _require(pairing in ("half", "neighbours"), f"{name} pair by halves or by neighbours")
-    if frequencies is None or dims == 0:
+    if frequencies is None or not dims:
         return None, 0
+    dims = int(dims)
     _device_tensor(frequencies, f"the frequencies of {name}", torch.float64, 1)
     _require(dims % 2 == 0 and 0 < dims <= most and frequencies.shape[0] >= dims // 2, f"the rotation does not fit {name}")
-    return frequencies, dims
+    _require(frequencies.get_device() == here, f"the frequencies of {name} lie on another device than the current one")
+    return frequencies.data_ptr(), dims
 
 
 def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_pages, v_pages, slots, positions, n_heads: int, n_kv_heads: int, dim: int, vdim: int, *, q_gain=None,
@@ -1585,39 +1589,32 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     tokens' codes rounded again). Tokens of a block behind those written stay as they are.
 
     Returns the queries [rows, n_heads * head_size] of ``out_dtype`` (default: the rows' type), zeros behind their ``dim`` elements (None without ``q_at``)."""
-    _, _, page_size, head_size = k_pages.shape
-    _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
-    _require(isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _DTYPE_CODE and (rows.stride(1) == 1 or rows.shape[1] == 1),
-             "the rows must be float32 or bfloat16 GPU rows with contiguous columns")
+    num_pages, _, page_size, head_size = k_pages.shape
+    here = _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
+    if not (isinstance(rows, torch.Tensor) and rows.is_cuda and rows.dim() == 2 and rows.dtype in _DTYPE_CODE and (rows.stride(1) == 1 or rows.shape[1] == 1)):
+        raise OperandError("the rows must be float32 or bfloat16 GPU rows with contiguous columns")
     n, width = rows.shape
-    _require(rows.stride(0) >= width or n <= 1, "the rows overlap")
+    stride = rows.stride(0)
+    _require(stride >= width or n <= 1, "the rows overlap")
+    _require(rows.get_device() == here, "the rows lie on another device than the current one")
     keeps, makes = k_at is not None, q_at is not None
     _require(keeps == (v_at is not None), "keys and values are kept together")
     _require(keeps or makes, "neither queries nor keys")
     _require(0 < dim <= head_size and 0 < vdim <= head_size, "the pages' heads are too small")
-    _require(n_heads > 0 and n_kv_heads > 0, "heads are at least one")
+    _require(n_heads > 0, "heads are at least one")
     _require(not makes or (0 <= q_at and q_at + n_heads * dim <= width), "the queries lie beyond the rows")
     _require(not keeps or (0 <= k_at and k_at + n_kv_heads * dim <= width and 0 <= v_at and v_at + n_kv_heads * vdim <= width), "keys or values lie beyond the rows")
-    for gain, name in ((q_gain, "q_gain"), (k_gain, "k_gain")):
-        if gain is not None:
-            _device_tensor(gain, name, torch.float32, 1)
-            _require(gain.shape[0] == dim, f"{name} does not match the heads")
-    frequencies, rot_dims = _rotation(frequencies, rot_dims, dim, pairing, "queries and keys")
-    v_frequencies, v_rot_dims = _rotation(v_frequencies, v_rot_dims, vdim, v_pairing, "values")
-    _device_tensor(positions, "positions", torch.int32, 1)
-    _require(positions.shape[0] >= n, "fewer positions than rows")
-    if keeps:
-        _device_tensor(slots, "slots", torch.int32, 1)
-        _require(slots.shape[0] >= n, "fewer slots than rows")
-        _require(k_pages.shape[0] * page_size <= 2**31, "the pages hold more tokens than a slot can name")
-    _one_device(rows, k_pages.codes, v_pages.codes, positions, slots if keeps else None, q_gain, k_gain, frequencies, v_frequencies)
+    q_gain, k_gain = _floats(q_gain, "q_gain", dim, here), _floats(k_gain, "k_gain", dim, here)
+    frequencies, rot_dims = _rotation(frequencies, rot_dims, dim, pairing, "queries and keys", here)
+    v_frequencies, v_rot_dims = _rotation(v_frequencies, v_rot_dims, vdim, v_pairing, "values", here)
+    position_at = _ints(positions, "positions", n, here)
+    slot_at = _ints(slots, "slots", n, here) if keeps else None
+    _require(num_pages * page_size <= 2**31, "the pages hold more tokens than a slot can name")
     out_dtype = out_dtype or rows.dtype
     q = torch.empty((n, n_heads * head_size), dtype=out_dtype, device=rows.device) if makes else None
-    check(library().mllm_scaled_append(_ptr(rows), rows.stride(0), int(q_at) if makes else -1, int(k_at) if keeps else -1, int(v_at) if keeps else -1, _ptr(q_gain), _ptr(k_gain),
-                                       float(eps), int(bool(unit)), _ptr(frequencies), rot_dims, int(pairing == "neighbours"), _ptr(v_frequencies), v_rot_dims,
-                                       int(v_pairing == "neighbours"), _ptr(positions), _ptr(slots if keeps else None), _ptr(q), _ptr(k_pages.codes), _ptr(k_pages.scales),
-                                       _ptr(v_pages.codes), _ptr(v_pages.scales), k_pages.shape[0], n, n_heads, n_kv_heads, int(dim), int(vdim), head_size, page_size,
-                                       _code(rows.dtype), _code(out_dtype), _stream()))
+    check(library().mllm_scaled_append(rows.data_ptr(), stride, q_at if makes else -1, k_at if keeps else -1, v_at if keeps else -1, q_gain, k_gain, eps, bool(unit), frequencies,
+                                       rot_dims, pairing == "neighbours", v_frequencies, v_rot_dims, v_pairing == "neighbours", position_at, slot_at, _ptr(q), *k_pages.addresses,
+                                       *v_pages.addresses, num_pages, n, n_heads, n_kv_heads, dim, vdim, head_size, page_size, _code(rows.dtype), _code(out_dtype), _stream()))
     return q
 
 
@@ -1625,13 +1622,13 @@ def scaled_rows(k_pages, v_pages, slots, out_dtype=torch.bfloat16):
     """What pages of 8 bits hold at ``slots`` (int32): (keys, values), each [len(slots), n_kv_heads, head_size] of ``out_dtype`` (bfloat16 holds them
     exactly); zeros where a slot is negative or lies behind the pages."""
     num_pages, n_kv_heads, page_size, head_size = k_pages.shape
-    _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
-    _device_tensor(slots, "slots", torch.int32, 1)
-    _one_device(k_pages.codes, v_pages.codes, slots)
+    here = _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
+    slot_at = _ints(slots, "slots", 0, here)
     n = slots.shape[0]
-    k, v = (torch.empty((n, n_kv_heads, head_size), dtype=out_dtype, device=slots.device) for _ in range(2))
-    check(library().mllm_scaled_rows(_ptr(k_pages.codes), _ptr(k_pages.scales), _ptr(v_pages.codes), _ptr(v_pages.scales), _ptr(slots), _ptr(k), _ptr(v), num_pages, n,
-                                     n_kv_heads, head_size, page_size, _code(out_dtype), _stream()))
+    both = torch.empty((2, n, n_kv_heads, head_size), dtype=out_dtype, device=slots.device)
+    k, v = both.unbind(0)
+    check(library().mllm_scaled_rows(*k_pages.addresses, *v_pages.addresses, slot_at, k.data_ptr(), v.data_ptr(), num_pages, n, n_kv_heads, head_size, page_size, _code(out_dtype),
+                                     _stream()))
     return k, v
 
 
@@ -1658,70 +1655,67 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
                       short_rows, short_requests, packed_out, softcap, sinks, chunk, keep_first, wide_out):
     """``paged_attention`` over pages of 8 bits: rows by themselves (decoding, short portions, batches without the shape of portions) a block per
     row and group of heads; portions a block per head and tile of rows."""
-    _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
+    here = _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
     num_pages, _, page_size, _ = k_pages.shape
     _require(n_heads > 0 and n_heads % n_kv_heads == 0, f"{n_heads} heads do not divide into {n_kv_heads} key/value heads")
-    width = n_heads * head_size
-    _strided_rows(q, "q", width)
-    if q.dtype not in _DTYPE_CODE:
-        raise OperandError(f"no kernel for element type {q.dtype}")
+    width, group = n_heads * head_size, n_heads // n_kv_heads
+    _strided_rows(q, "q", width, here)
+    code = _code(q.dtype)
     n = q.shape[0]
-    _device_tensor(block_tables, "block_tables", torch.int32, 2)
-    _require(block_tables.shape[0] > 0 and block_tables.shape[1] > 0, "block tables without entries")
+    if not (isinstance(block_tables, torch.Tensor) and block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.get_device() == here and block_tables.is_contiguous()):
+        _device_tensor(block_tables, "block_tables", torch.int32, 2)
+        raise OperandError("block_tables lie on another device than the current one")
+    n_tables, max_blocks = block_tables.shape
+    _require(n_tables > 0 and max_blocks > 0, "block tables without entries")
     _require(window >= 0 and chunk >= 0 and not (chunk and window), "the keys a row sees are bounded by a window or by chunks, not both")
     keep = keep_first if window else 0
     _require(keep >= 0, "kept first keys are a number of them")
     _require(not (wide_out and packed_out), "rows in the packed layout leave in the queries' type")
-    if sinks is not None:
-        _device_tensor(sinks, "sinks", torch.float32, 1)
-        _require(sinks.shape[0] == n_heads, "one sink a head")
+    sink_at = _floats(sinks, "sinks", n_heads, here)
     out_dtype = torch.float32 if wide_out else q.dtype
     if out is None:
         out = torch.empty((n, width), dtype=out_dtype, device=q.device)
-    _strided_rows(out, "out", width)
-    _require(out.dtype == out_dtype and out.shape[0] == n, "out has the wrong shape or type")
-    _device_tensor(token_request, "token_request", torch.int32, 1)
-    _device_tensor(positions, "positions", torch.int32, 1)
-    _require(token_request.shape[0] >= n and positions.shape[0] >= n, "fewer positions than rows")
-    _one_device(q, out, k_pages.codes, v_pages.codes, token_request, positions, block_tables, sinks, q_starts, context_lens)
+    else:
+        _strided_rows(out, "out", width, here)
+        _require(out.dtype == out_dtype and out.shape[0] == n, "out has the wrong shape or type")
+    request_at, position_at = _ints(token_request, "token_request", n, here), _ints(positions, "positions", n, here)
     lib = library()
     if n == 0:
         return out
-    reach = block_tables.shape[1] * page_size
-    pages = (_ptr(k_pages.codes), _ptr(k_pages.scales), _ptr(v_pages.codes), _ptr(v_pages.scales))
+    table_at = block_tables.data_ptr()
+    given = (q.data_ptr(), q.stride(0), *k_pages.addresses, *v_pages.addresses)
 
     def rows_alone(count, into, packed):
+        reach = max_blocks * page_size
         span = min(window + keep if window else chunk or reach, reach)
         tiles = -(-span // SCALED_TILE) + (2 if window or chunk else 0)
-        sets = -(-(n_heads // n_kv_heads) // 16)
-        longest = tiles if max_len is None else max(1, min(tiles, -(-int(max_len) // SCALED_TILE)))
-        waves, run, runs = scaled_cut(count * n_kv_heads * sets, longest, head_size, min(16, n_heads // n_kv_heads), q.dtype == torch.float32)
+        if max_len is not None:   # (what lies beyond it is the last run's)
+            tiles = max(1, min(tiles, -(-int(max_len) // SCALED_TILE)))
+        waves, run, runs = scaled_cut(count * n_kv_heads * -(-group // 16), tiles, head_size, min(16, group), code == F32)
         parts = torch.empty((count, n_heads, runs, head_size + 2), dtype=torch.float32, device=q.device) if runs > 1 else None
-        check(lib.mllm_scaled_attention_rows(_ptr(q), q.stride(0), *pages, _ptr(into), width if packed else into.stride(0), _ptr(token_request), _ptr(positions),
-                                             _ptr(block_tables), block_tables.shape[1], block_tables.shape[0], num_pages, count, n_heads, n_kv_heads, head_size, page_size, window,
-                                             scale, _code(q.dtype), softcap, _ptr(sinks), chunk, keep, int(wide_out), int(packed), waves, run, runs, _ptr(parts), _stream()))
+        check(lib.mllm_scaled_attention_rows(*given, into.data_ptr(), width if packed else into.stride(0), request_at, position_at, table_at, max_blocks, n_tables, num_pages, count,
+                                             n_heads, n_kv_heads, head_size, page_size, window, scale, code, softcap, sink_at, chunk, keep, wide_out, packed, waves, run, runs,
+                                             _ptr(parts), _stream()))
 
-    portions = max_q_len is not None and max_q_len > SCALED_SHORT and q_starts is not None and context_lens is not None
-    if not portions:
+    if not (max_q_len is not None and max_q_len > SCALED_SHORT and q_starts is not None and context_lens is not None):
         if packed_out:
             result = empty_packed_rows(n, width, q.dtype, q.device)
             rows_alone(n, result.data, True)
             return result
         rows_alone(n, out, False)
         return out
-    _device_tensor(q_starts, "q_starts", torch.int32, 1)
-    _device_tensor(context_lens, "context_lens", torch.int32, 1)
     n_requests = context_lens.shape[0]
     _require(q_starts.shape[0] == n_requests + 1, "q_starts must have one entry more than context_lens")
-    _require(block_tables.shape[0] >= n_requests, "fewer block tables than requests")
+    _require(n_tables >= n_requests, "fewer block tables than requests")
+    start_at, context_at = _ints(q_starts, "q_starts", n_requests + 1, here), _ints(context_lens, "context_lens", n_requests, here)
     skipped = 0
     if short_rows is not None and short_requests is not None and 0 < short_rows < n:
         _require(0 < short_requests < n_requests, "short_requests does not cut the batch in two")
         rows_alone(int(short_rows), out, False)
         skipped = int(short_requests)
-    check(lib.mllm_scaled_attention_tiles(_ptr(q), q.stride(0), *pages, _ptr(out), out.stride(0), _ptr(q_starts[skipped:]), _ptr(context_lens[skipped:]), _ptr(block_tables[skipped:]),
-                                          block_tables.shape[1], n_requests - skipped, num_pages, n, int(max_q_len), n_heads, n_kv_heads, head_size, page_size, window, scale,
-                                          _code(q.dtype), softcap, _ptr(sinks), chunk, keep, int(wide_out), _stream()))
+    check(lib.mllm_scaled_attention_tiles(*given, out.data_ptr(), out.stride(0), start_at + 4 * skipped, context_at + 4 * skipped, table_at + 4 * skipped * max_blocks, max_blocks,
+                                          n_requests - skipped, num_pages, n, int(max_q_len), n_heads, n_kv_heads, head_size, page_size, window, scale, code, softcap, sink_at, chunk,
+                                          keep, wide_out, _stream()))
     return out
 
 
