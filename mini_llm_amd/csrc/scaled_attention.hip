@@ -19,7 +19,7 @@ struct AttendArguments {
     const int* block_tables;
     const float* sinks;
     ScaledPlanes planes;
-    int max_blocks, n_tables, n_rows, n_heads, window, chunk, keep, aligned, negative, wide_out, out_packed;
+    int max_blocks, n_tables, n_rows, n_heads, window, chunk, keep, aligned, negative, wide_out, out_packed, out_aligned;
     ScoreScale scale;
     float sink_factor;   // log2 e where weights are powers of two
 };
@@ -30,6 +30,24 @@ __device__ __forceinline__ void put_result(const AttendArguments& a, int row, in
     const size_t index = a.out_packed ? packed_element<T>(row, at, a.n_heads * a.planes.head_size) : (size_t)row * a.out_stride + at;
     if (sizeof(T) == 4 || !a.wide_out) static_cast<T*>(a.out)[index] = from_float<T>(value);
     else static_cast<float*>(a.out)[index] = value;
+}
+
+// Four neighbouring results of a row that is not packed.
+template <typename T>
+__device__ __forceinline__ void put_four(const AttendArguments& a, int row, int at, f32x4 value) {
+    const size_t index = (size_t)row * a.out_stride + at;
+    if (sizeof(T) == 4 || a.wide_out) {
+        float* const to = static_cast<float*>(a.out) + index;
+        if (a.out_aligned) *reinterpret_cast<f32x4*>(to) = value;
+        else
+            for (int e = 0; e < 4; e++) to[e] = value[e];
+    } else {
+        bf16_t* const to = static_cast<bf16_t*>(a.out) + index;
+        const bf16x4 rounded = {static_cast<bf16_t>(value[0]), static_cast<bf16_t>(value[1]), static_cast<bf16_t>(value[2]), static_cast<bf16_t>(value[3])};
+        if (a.out_aligned) *reinterpret_cast<bf16x4*>(to) = rounded;
+        else
+            for (int e = 0; e < 4; e++) to[e] = rounded[e];
+    }
 }
 
 // What a row sees, or no tile at all.
@@ -153,8 +171,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention
     constexpr bool WIDE = sizeof(T) == 4;
     typedef ScaledSweep<HD, CT, WIDE, true, WHOLE> Sweep;
     constexpr int ROWS = 16 * CT, WAVES = 4;
-    __shared__ float meeting[WAVES / 2][CT][Sweep::DT + 1][4][WAVE];   // what half of the waves hold, lane by lane
-    __shared__ bf16x8 queries[Sweep::Q_PIECES];
+    // the queries' operands while keys are walked; then what the waves hold, row by row
+    constexpr int PITCH = HD + 4;
+    __shared__ union {
+        bf16x8 queries[Sweep::Q_PIECES];
+        float meeting[WAVES][ROWS][PITCH];
+    } lds;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int request = blockIdx.z, head = blockIdx.y, head_size = a.planes.head_size;
     const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
@@ -173,60 +195,48 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention
         const bool valid = local < q_len;
         if (ct % WAVES == wave) {
             sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
-            sweep.share_query(ct, queries, lane);
+            sweep.share_query(ct, lds.queries, lane);
         }
     }
-    sweep.q_shared = queries;
+    sweep.q_shared = lds.queries;
     __syncthreads();
     const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
     sweep.tiles(range, wave, WAVES, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale,
                 {context + row0 + lane % 16, position1, a.window, a.chunk, a.keep}, scaled_first_key(position1, a.window, a.chunk), position0, lane);
 
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) sweep.l[ct] = sweep.weight_sum(ct);
-    // the waves' sums: the upper half's into the lower half's, then wave 1's into wave 0's
-#pragma unroll
-    for (int half = WAVES / 2; half >= 1; half /= 2) {
-        __syncthreads();
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-#pragma unroll
-                for (int dt = 0; dt < Sweep::DT; dt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) meeting[wave - half][ct][dt][i][lane] = sweep.o[ct][dt][i];
-                meeting[wave - half][ct][Sweep::DT][0][lane] = sweep.m[ct];
-                meeting[wave - half][ct][Sweep::DT][1][lane] = sweep.l[ct];
-            }
-        }
-        __syncthreads();
-        if (wave < half) {
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                const float other = meeting[wave][ct][Sweep::DT][0][lane], top = fmaxf(sweep.m[ct], other);
-                const float mine = weight_of<WIDE>(sweep.m[ct] - top), theirs = weight_of<WIDE>(other - top);
-                sweep.m[ct] = top;
-                sweep.l[ct] = sweep.l[ct] * mine + meeting[wave][ct][Sweep::DT][1][lane] * theirs;
-#pragma unroll
-                for (int dt = 0; dt < Sweep::DT; dt++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sweep.o[ct][dt][i] = sweep.o[ct][dt][i] * mine + meeting[wave][ct][dt][i][lane] * theirs;
-            }
-        }
-    }
-    if (wave != 0) return;
+    __syncthreads();   // (all waves are through with the queries)
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const int local = row0 + 16 * ct + lane % 16;
-        if (local >= q_len) continue;
-        float total = sweep.l[ct];
-        if (a.sinks) total += weight_of<WIDE>(a.sinks[head] * a.sink_factor - sweep.m[ct]);
+        float* const mine = lds.meeting[wave][16 * ct + lane % 16];
+#pragma unroll
+        for (int dt = 0; dt < Sweep::DT; dt++) *reinterpret_cast<f32x4*>(mine + 16 * dt + 4 * (lane / 16)) = sweep.o[ct][dt];
+        const float sum = sweep.weight_sum(ct);
+        if (lane < 16) {
+            mine[HD] = sweep.m[ct];
+            mine[HD + 1] = sum;
+        }
+    }
+    __syncthreads();
+    // four elements of a row a thread, as they lie in the results
+    const int fours = head_size / 4;
+    for (int i = threadIdx.x; i < ROWS * fours; i += blockDim.x) {
+        const int row = i / fours, d = 4 * (i % fours);
+        if (row0 + row >= q_len) break;
+        float top = NO_SCORE;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) top = fmaxf(top, lds.meeting[w][row][HD]);
+        float total = a.sinks ? weight_of<WIDE>(a.sinks[head] * a.sink_factor - top) : 0.0f;
+        f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const float factor = weight_of<WIDE>(lds.meeting[w][row][HD] - top);
+            total += lds.meeting[w][row][HD + 1] * factor;
+            const f32x4 theirs = *reinterpret_cast<const f32x4*>(&lds.meeting[w][row][d]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) value[e] += theirs[e] * factor;
+        }
         const float inverse = 1.0f / total;
-#pragma unroll
-        for (int dt = 0; dt < Sweep::DT; dt++)
-            if (dt * 16 < head_size)
-#pragma unroll
-                for (int i = 0; i < 4; i++) put_result<T>(a, q_first + local, head * head_size + dt * 16 + 4 * (lane / 16) + i, sweep.o[ct][dt][i] * inverse);
+        put_four<T>(a, q_first + row0 + row, head * head_size + d, value * inverse);
     }
 }
 
@@ -255,6 +265,8 @@ AttendArguments attend_arguments(const void* q, long long q_stride, const void* 
     a.planes = {(const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales, num_pages, n_kv_heads, head_size, shift};
     a.max_blocks = max_blocks, a.n_tables = n_tables, a.n_rows = n_rows, a.n_heads = n_heads, a.window = window, a.chunk = chunk, a.keep = keep;
     a.aligned = (uintptr_t)q % 16 == 0 && q_stride * (dtype == MLLM_F32 ? 4 : 2) % 16 == 0;
+    const int out_size = dtype == MLLM_F32 || wide_out ? 4 : 2;
+    a.out_aligned = (uintptr_t)out % (4 * out_size) == 0 && out_stride % 4 == 0;   // four results at a time
     a.negative = scale < 0.0f, a.wide_out = wide_out;
     // (a factor of zero would make numbers that are none of masked scores: 1e-30 leaves as little between any two others)
     a.scale = {size * unit > 1e-30f ? size * unit : 1e-30f, softcap > 0.0f ? size / softcap : 0.0f, softcap > 0.0f ? softcap * unit : 0.0f};

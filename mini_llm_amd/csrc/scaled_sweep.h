@@ -66,10 +66,18 @@ struct ScoreScale {
     float cap_in, cap;  // cap > 0: score <- cap tanh(raw cap_in), cap times log2 e where weights are powers of two
 };
 
+// 2^x for scores in units of log2 e; in 32-bit e^x: with t = x log2 e as rounded and r what that leaves, 2^t (1 + r ln 2), the hardware's 2^t
+// and a handful of instructions more, within two units in the last place.
 template <bool WIDE>
 __device__ __forceinline__ float weight_of(float x) {
-    if constexpr (WIDE) return expf(x);
-    else return __builtin_amdgcn_exp2f(x);
+    if constexpr (!WIDE) return __builtin_amdgcn_exp2f(x);
+    else {
+        const float t = x * 1.44269504f;
+        const float r = __builtin_fmaf(x, 1.44269504f, -t) + x * 1.9259629911e-8f;   // (log2 e in two pieces)
+        const float power = __builtin_amdgcn_exp2f(t);
+        // (an x of minus infinity leaves no number in r, and a power of zero says what it is)
+        return power > 0.0f ? __builtin_fmaf(power, r * 0.69314718f, power) : power;
+    }
 }
 
 // APART: the columns are rows at positions of their own (else heads of one row, which see the same keys). WHOLE: pages of 64 tokens or more, so a
@@ -271,16 +279,17 @@ struct ScaledSweep {
                     }
             }
             if constexpr (MASKED) {
-                seen[ct] = 0;
+                // bit 4 t + i: whether key + 4 t + i counts
                 const int last = min(columns.position + 16 * ct, columns.most), first = scaled_first_key(last, columns.window, columns.chunk);
+                auto below = [&](int end) { return (1u << min(max(end - key, 0), BLOCK_TOKENS)) - 1u; };   // keys below `end`
+                seen[ct] = below(last + 1) & (~below(first) | below(columns.keep));
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int k = key + 4 * t + i;
-                        const bool counts = k <= last && (k >= first || k < columns.keep);
-                        seen[ct] |= counts ? 1u << (4 * t + i) : 0u;
-                        s[ct][t][i] = counts ? s[ct][t][i] : -INFINITY;
+                        const float score = s[ct][t][i];   // (bits are taken of a number by itself: of a vector's element they come out as the first one's)
+                        const uint32_t mask = (uint32_t)((int)(seen[ct] << (31 - 4 * t - i)) >> 31), bits = __builtin_bit_cast(uint32_t, score);
+                        s[ct][t][i] = __builtin_bit_cast(float, (bits & mask) | (0xff800000u & ~mask));
                     }
             }
             float best = s[ct][0][0];
