@@ -63,8 +63,13 @@ struct RowView {
     __device__ __forceinline__ bool sees() const { return request >= 0 && position >= 0; }
 };
 
+constexpr int MOST_RUNS = 1024;   // of a row: their factors lie in LDS when they are put together
+
 // The most waves a block of rows may have: as many as have the registers they need.
 constexpr int rows_waves(int padded, int size) { return padded == 64 ? (size == 2 ? 16 : 8) : 1024 / padded; }
+
+// How many runs a row's tiles are cut into.
+__device__ __forceinline__ int runs_of(int tiles, int run_tiles, int n_runs) { return min(ceil_div(tiles, run_tiles), n_runs); }
 
 // Rows by themselves (decoding, short portions, and whatever else comes without the shape of portions): a block per row, group of up to 16
 // heads that share a key/value head, and run of `run_tiles` tiles; its waves take the run's tiles in turn and meet in LDS. Rows of more
@@ -87,9 +92,10 @@ __global__ __launch_bounds__(WAVE * rows_waves(HD, sizeof(T))) void scaled_rows_
         return;
     }
     const TileRange range(view.first, view.position, a.keep);
-    const int begin = run * run_tiles, end = run == n_runs - 1 ? range.count : min(range.count, begin + run_tiles);
-    if (begin >= end) return;
-    const bool alone = n_runs == 1 || range.count <= run_tiles;
+    const int runs = runs_of(range.count, run_tiles, n_runs);
+    if (run >= runs) return;
+    const bool alone = runs == 1;
+    const int share = ceil_div(range.count, runs), begin = run * share, end = min(range.count, begin + share);   // (the runs of a row are alike)
 
     Sweep sweep;
     sweep.init(head_size, lane);
@@ -138,28 +144,44 @@ __global__ __launch_bounds__(WAVE * rows_waves(HD, sizeof(T))) void scaled_rows_
     }
 }
 
-// Puts the runs of a row's head together: a block a (row, head).
+// Puts the runs of a row's head together: a wave a (row, head), four to a block; eight runs' sums are on their way at a time.
 template <typename T>
-__global__ __launch_bounds__(64) void scaled_merge_kernel(AttendArguments a, int run_tiles, int n_runs, const float* __restrict__ parts) {
+__global__ __launch_bounds__(256) void scaled_merge_kernel(AttendArguments a, int run_tiles, int n_runs, const float* __restrict__ parts) {
     constexpr bool WIDE = sizeof(T) == 4;
-    const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, head_size = a.planes.head_size;
+    extern __shared__ float factors[];   // [wave][n_runs]
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int row = blockIdx.x, head = blockIdx.y * 4 + wave, head_size = a.planes.head_size;
+    if (head >= a.n_heads) return;
     const RowView view(a, row);
     if (!view.sees()) return;
     const TileRange range(view.first, view.position, a.keep);
-    if (range.count <= run_tiles) return;
-    const int runs = min(ceil_div(range.count, run_tiles), n_runs);
-    const float* const mine = parts + ((size_t)row * a.n_heads + head) * n_runs * (head_size + 2);
+    const int runs = runs_of(range.count, run_tiles, n_runs);
+    if (runs == 1) return;
     const int pitch = head_size + 2;
+    const float* const mine = parts + ((size_t)row * a.n_heads + head) * n_runs * pitch;
+    float* const factor = factors + wave * n_runs;
     float top = NO_SCORE;
     for (int r = lane; r < runs; r += WAVE) top = fmaxf(top, mine[r * pitch + head_size]);
     top = wave_max_total(top);
     float total = 0.0f;
-    for (int r = lane; r < runs; r += WAVE) total += mine[r * pitch + head_size + 1] * weight_of<WIDE>(mine[r * pitch + head_size] - top);
+    for (int r = lane; r < runs; r += WAVE) {
+        const float f = weight_of<WIDE>(mine[r * pitch + head_size] - top);
+        factor[r] = f;
+        total += mine[r * pitch + head_size + 1] * f;
+    }
     total = wave_total(total);
     if (a.sinks) total += weight_of<WIDE>(a.sinks[head] * a.sink_factor - top);
+    __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // (the wave's own factors, by its other lanes)
+    __builtin_amdgcn_wave_barrier();
     for (int d = lane; d < head_size; d += WAVE) {
         float value = 0.0f;
-        for (int r = 0; r < runs; r++) value += mine[r * pitch + d] * weight_of<WIDE>(mine[r * pitch + head_size] - top);
+        for (int r0 = 0; r0 < runs; r0 += 8) {
+            float part[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) part[u] = mine[min(r0 + u, runs - 1) * pitch + d];
+#pragma unroll
+            for (int u = 0; u < 8; u++) value += r0 + u < runs ? part[u] * factor[min(r0 + u, runs - 1)] : 0.0f;
+        }
         put_result<T>(a, row, head * head_size + d, value / total);
     }
 }
@@ -276,8 +298,8 @@ AttendArguments attend_arguments(const void* q, long long q_stride, const void* 
 
 }  // namespace
 
-// Rows by themselves. The keys of a row are cut into runs of run_tiles tiles of 64, n_runs of them at most: a shorter sequence has fewer, and
-// the last run of a longer one takes all that is left; n_runs > 1 needs `parts`, n_rows * n_heads * n_runs * (head_size + 2) floats.
+// Rows by themselves. The keys of a row are cut into as many runs as have at most run_tiles tiles of 64 each, n_runs at most (a longer
+// sequence has longer runs, so no key is left out); n_runs > 1 needs `parts`, n_rows * n_heads * n_runs * (head_size + 2) floats.
 MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales, void* out,
                                         long long out_stride, const int* token_request, const int* positions, const int* block_tables, int max_blocks, int n_tables,
                                         int num_pages, int n_rows, int n_heads, int n_kv_heads, int head_size, int page_size, int window, float scale, int dtype,
@@ -288,7 +310,7 @@ MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const
     a.token_request = token_request, a.positions = positions, a.out_packed = out_packed;
     if (int status = refuse_attend("scaled_attention_rows", a, page_size, dtype)) return status;
     const int padded = head_size <= 64 ? 64 : head_size <= 128 ? 128 : 256, most = rows_waves(padded, dtype == MLLM_F32 ? 4 : 2);
-    MLLM_REQUIRE(waves >= 1 && waves <= most && run_tiles >= 1 && n_runs >= 1 && n_runs <= 65535 && (n_runs == 1 || parts != nullptr),
+    MLLM_REQUIRE(waves >= 1 && waves <= most && run_tiles >= 1 && n_runs >= 1 && n_runs <= MOST_RUNS && (n_runs == 1 || parts != nullptr),
                  "scaled_attention_rows: %d waves (1..%d), runs of %d tiles, %d runs (with memory for more than one)", waves, most, run_tiles, n_runs);
     const int group = n_heads / n_kv_heads, columns = group < 16 ? group : 16;
     const size_t lds = (size_t)waves * columns * (head_size + 4) * sizeof(float);
@@ -314,8 +336,10 @@ MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const
     if (int status = mllm_check_launch("scaled_attention_rows")) return status;
     if (n_runs == 1) return 0;
     mllm_count_kernel(MLLM_K_SCALED_ATTENTION_MERGE);
-    if (dtype == MLLM_F32) scaled_merge_kernel<float><<<dim3(n_rows, n_heads), WAVE, 0, stream>>>(a, run_tiles, n_runs, parts);
-    else scaled_merge_kernel<bf16_t><<<dim3(n_rows, n_heads), WAVE, 0, stream>>>(a, run_tiles, n_runs, parts);
+    const dim3 merge_grid(n_rows, ceil_div(n_heads, 4));
+    const size_t merge_lds = (size_t)4 * n_runs * sizeof(float);
+    if (dtype == MLLM_F32) scaled_merge_kernel<float><<<merge_grid, 4 * WAVE, merge_lds, stream>>>(a, run_tiles, n_runs, parts);
+    else scaled_merge_kernel<bf16_t><<<merge_grid, 4 * WAVE, merge_lds, stream>>>(a, run_tiles, n_runs, parts);
     return mllm_check_launch("scaled_attention_merge");
 }
 

@@ -2,9 +2,13 @@
 // and turned by their positions, keys and values put into their blocks; and what a cache holds, read back.
 #include "scaled_blocks.h"
 
+#include <algorithm>
+
 namespace {
 
-constexpr int APPEND_BLOCKS = 1024;   // blocks of threads that a call is shared among, if it has the heads for them
+// Blocks of threads that a call is shared among, if it has the heads for them: 8,192 rows of 32 + 16 heads of 128, with reading back, us with 512 / 1,024 / 1,536 / 2,048 /
+// 3,072: 90 / 72 / 72 / 75 / 77 (each block makes its run's cosines again); 5,000 rows of the same in 32-bit 109 / 99 / 97 / 95 / 98.
+constexpr int APPEND_BLOCKS = 1536;
 
 // What is done to the heads of one kind on their way.
 struct Turn {
@@ -52,12 +56,10 @@ __device__ __forceinline__ void turn_of(int position, double frequency, double& 
 // A 64-bit number in 32 with its last bit set where anything was cut off (rounding to odd): rounded again to fewer bits it gives what the
 // 64-bit number does.
 __device__ __forceinline__ float sticky(double x) {
-    float f = (float)x;
+    const float f = (float)x;
     const double back = (double)f;
-    if (back == x || x != x) return f;
-    uint32_t bits = __builtin_bit_cast(uint32_t, f);
-    if (fabs(back) > fabs(x)) bits--;
-    return __builtin_bit_cast(float, bits | 1u);
+    const uint32_t bits = __builtin_bit_cast(uint32_t, f) - (fabs(back) > fabs(x) ? 1u : 0u);
+    return __builtin_bit_cast(float, bits | (back != x ? 1u : 0u));   // (what is no number stays so)
 }
 
 // A run of rows that fall into one block, as a block of threads takes it.
@@ -82,6 +84,15 @@ struct BlockScale {
         grown = lead > 0 && exponent > old;
     }
 };
+
+// The cosines and sines of a run's positions, [16][pitch] pairs: in 64 bits for what is rounded to 8 bits, in 32 for queries. A row is a pair longer
+// than it needs to be: the lanes of a wave read the same pair of 16 rows, which would lie on the same banks.
+struct TurnTable {
+    const double2* wide;
+    const float2* narrow;
+    int pairs, pitch;   // pairs 0: nothing turns
+};
+__host__ __device__ __forceinline__ int turn_pitch(int pairs) { return pairs ? pairs + 1 : 0; }
 
 // Where the pair of element d lies, its number, and whether d is the first of the two.
 __device__ __forceinline__ int partner_of(const Turn& turn, int d, int& pair, bool& is_first) {
@@ -111,7 +122,7 @@ __device__ __forceinline__ void rescale_keys(uint8_t* codes, int head_size, int 
 // A head's values of a run, by a wave: a lane has elements lane, lane + 64, .. of every row, so that what it makes of one is the 16 tokens'
 // codes that lie together.
 template <typename T, int E>
-__device__ __forceinline__ void append_values(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+__device__ __forceinline__ void append_values(const AppendArguments& a, const Run& run, int head, const TurnTable& turns, int lane) {
     const size_t block = run.block_in_head + head * run.head_blocks;
     uint8_t* const codes = a.v_codes + block * BLOCK_TOKENS * a.head_size;
     const T* const from = static_cast<const T*>(a.rows) + (size_t)run.first * a.stride + a.v_at + head * a.vdim;
@@ -121,12 +132,18 @@ __device__ __forceinline__ void append_values(const AppendArguments& a, const Ru
 #pragma unroll
     for (int e = 0; e < E; e++) {
         const int d = lane + e * WAVE;
+        const T* at = from + min(d, a.vdim - 1);   // (a row and an element that are there, whether they count or not: nothing waits for a branch)
 #pragma unroll
-        for (int t = 0; t < BLOCK_TOKENS; t++) x[t][e] = t < run.count && d < a.vdim ? to_float(from[t * a.stride + d]) : 0.0f;
+        for (int t = 0; t < BLOCK_TOKENS; t++) {
+            x[t][e] = to_float(*at);
+            at += t + 1 < run.count ? a.stride : 0;
+        }
+#pragma unroll
+        for (int t = 0; t < BLOCK_TOKENS; t++) x[t][e] = t < run.count && d < a.vdim ? x[t][e] : 0.0f;
         piece[e] = Vec16{{0u, 0u, 0u, 0u}};
         if (run.count < BLOCK_TOKENS && d < a.head_size) piece[e] = *reinterpret_cast<const Vec16*>(codes + d * BLOCK_TOKENS);
     }
-    if (pairs) {
+    if (turns.pairs) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const int d = lane + e * WAVE;
@@ -135,8 +152,10 @@ __device__ __forceinline__ void append_values(const AppendArguments& a, const Ru
                 bool is_first;
                 const int other = partner_of(a.v_turn, d, pair, is_first);
 #pragma unroll
-                for (int t = 0; t < BLOCK_TOKENS; t++)
-                    if (t < run.count) x[t][e] = turned_once(x[t][e], to_float(from[t * a.stride + other]), is_first, turns[t * pairs + pair]);
+                for (int t = 0; t < BLOCK_TOKENS; t++) {
+                    if (t < run.count) x[t][e] = turned_once(x[t][e], to_float(from[t * a.stride + other]), is_first, turns.wide[t * turns.pitch + pair]);
+                    __builtin_amdgcn_sched_barrier(0);   // (all tokens' 64-bit numbers at once would not fit the registers)
+                }
             }
         }
     }
@@ -192,7 +211,7 @@ struct HeadPieces {
         second = apart ? 8 * unit + turn.dims / 2 : 16 * unit + 8;
     }
 
-    __device__ __forceinline__ void load(const AppendArguments& a, const Run& run, int column, const float* gain, const double2* turns, int pairs, int lane) {
+    __device__ __forceinline__ void load(const AppendArguments& a, const Run& run, int column, const float* gain, const TurnTable& turns, int lane) {
         const int token = lane % 16;
         const T* const from = static_cast<const T*>(a.rows) + (size_t)(run.first + (token < run.count ? token : 0)) * a.stride + column;
         float sum = 0.0f;
@@ -232,32 +251,41 @@ struct HeadPieces {
                     for (int i = 0; i < 8; i++) x[e][p][i] *= factor * (gain != nullptr && 16 * unit < a.dim ? gain[at[p] + i] : 1.0f);
             }
         }
-        if (!pairs) return;
+        if (!turns.pairs) return;
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const int unit = 4 * e + lane / 16;
             if (16 * unit >= a.turn.dims || token >= run.count) continue;
-            const double2* const mine = turns + token * pairs;
+            const auto* const mine = table_of(turns) + token * turns.pitch;
             if (a.turn.neighbours) {
 #pragma unroll
                 for (int p = 0; p < 2; p++)
 #pragma unroll
-                    for (int i = 0; i < 8; i += 2) turn_pair(x[e][p][i], x[e][p][i + 1], mine[8 * unit + 4 * p + i / 2]);
+                    for (int i = 0; i < 8; i += 2) {
+                        turn_pair(x[e][p][i], x[e][p][i + 1], mine[8 * unit + 4 * p + i / 2]);
+                        if (KEYS && i % 4 == 2) __builtin_amdgcn_sched_barrier(0);
+                    }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i++) turn_pair(x[e][0][i], x[e][1][i], mine[8 * unit + i]);
+                for (int i = 0; i < 8; i++) {
+                    turn_pair(x[e][0][i], x[e][1][i], mine[8 * unit + i]);
+                    if (KEYS && i % 2 == 1) __builtin_amdgcn_sched_barrier(0);   // (all pairs' 64-bit numbers at once would take half the registers)
+                }
             }
         }
     }
 
+    static __device__ __forceinline__ auto table_of(const TurnTable& turns) {
+        if constexpr (KEYS) return turns.wide;
+        else return turns.narrow;
+    }
     static __device__ __forceinline__ void turn_pair(float& u, float& v, double2 cs) {
-        if constexpr (KEYS) {
-            const float a = turned_once(u, v, true, cs), b = turned_once(v, u, false, cs);
-            u = a, v = b;
-        } else {
-            const float c = (float)cs.x, s = (float)cs.y, a = u * c - v * s, b = v * c + u * s;
-            u = a, v = b;
-        }
+        const float a = turned_once(u, v, true, cs), b = turned_once(v, u, false, cs);
+        u = a, v = b;
+    }
+    static __device__ __forceinline__ void turn_pair(float& u, float& v, float2 cs) {
+        const float a = u * cs.x - v * cs.y, b = v * cs.x + u * cs.y;
+        u = a, v = b;
     }
 };
 
@@ -271,9 +299,9 @@ __device__ __forceinline__ void store_eight(O* to, const float (&x)[8]) {
 }
 
 template <typename T, int E>
-__device__ __forceinline__ void queries_in_pieces(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+__device__ __forceinline__ void queries_in_pieces(const AppendArguments& a, const Run& run, int head, const TurnTable& turns, int lane) {
     HeadPieces<T, E, false> pieces;
-    pieces.load(a, run, a.q_at + head * a.dim, a.q_gain, turns, pairs, lane);
+    pieces.load(a, run, a.q_at + head * a.dim, a.q_gain, turns, lane);
     const int token = lane % 16;
     if (token >= run.count) return;
 #pragma unroll
@@ -292,12 +320,12 @@ __device__ __forceinline__ void queries_in_pieces(const AppendArguments& a, cons
 }
 
 template <typename T, int E>
-__device__ __forceinline__ void keys_in_pieces(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+__device__ __forceinline__ void keys_in_pieces(const AppendArguments& a, const Run& run, int head, const TurnTable& turns, int lane) {
     const size_t block = run.block_in_head + head * run.head_blocks;
     uint8_t* const codes = a.k_codes + block * BLOCK_TOKENS * a.head_size;
     const float held = a.k_scales[block];
     HeadPieces<T, E, true> pieces;
-    pieces.load(a, run, a.k_at + head * a.dim, a.k_gain, turns, pairs, lane);
+    pieces.load(a, run, a.k_at + head * a.dim, a.k_gain, turns, lane);
     float largest = 0.0f;
 #pragma unroll
     for (int e = 0; e < E; e++)
@@ -328,7 +356,7 @@ __device__ __forceinline__ void keys_in_pieces(const AppendArguments& a, const R
 
 // The same an element a lane, for heads and places that are no whole pieces: a row's query head ..
 template <typename T, int E>
-__device__ __forceinline__ void query_by_elements(const AppendArguments& a, const Run& run, int row, int head, const double2* turns, int pairs, int lane) {
+__device__ __forceinline__ void query_by_elements(const AppendArguments& a, const Run& run, int row, int head, const TurnTable& turns, int lane) {
     const T* const from = static_cast<const T*>(a.rows) + (size_t)(run.first + row) * a.stride + a.q_at + head * a.dim;
     const bool normed = a.q_gain != nullptr || a.unit;
     float x[E], factor = 1.0f, sum = 0.0f;
@@ -343,12 +371,12 @@ __device__ __forceinline__ void query_by_elements(const AppendArguments& a, cons
     for (int e = 0; e < E; e++) {
         const int d = lane + e * WAVE;
         float value = d < a.dim ? weighted(x[e], d) : 0.0f;
-        if (pairs && d < a.turn.dims) {
+        if (turns.pairs && d < a.turn.dims) {
             int pair;
             bool is_first;
             const int other = partner_of(a.turn, d, pair, is_first);
-            const double2 cs = turns[row * pairs + pair];
-            value = value * (float)cs.x + weighted(to_float(from[other]), other) * (is_first ? -(float)cs.y : (float)cs.y);
+            const float2 cs = turns.narrow[row * turns.pitch + pair];
+            value = value * cs.x + weighted(to_float(from[other]), other) * (is_first ? -cs.y : cs.y);
         }
         const size_t to = ((size_t)(run.first + row) * a.n_heads + head) * a.head_size + d;
         if (d < a.head_size) {
@@ -360,7 +388,7 @@ __device__ __forceinline__ void query_by_elements(const AppendArguments& a, cons
 
 // .. and a head's keys of a run.
 template <typename T, int E>
-__device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const Run& run, int head, const double2* turns, int pairs, int lane) {
+__device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const Run& run, int head, const TurnTable& turns, int lane) {
     const size_t block = run.block_in_head + head * run.head_blocks;
     uint8_t* const codes = a.k_codes + block * BLOCK_TOKENS * a.head_size;
     const T* const from = static_cast<const T*>(a.rows) + (size_t)run.first * a.stride + a.k_at + head * a.dim;
@@ -382,11 +410,11 @@ __device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const
             const int d = lane + e * WAVE;
             if (t < run.count && d < a.dim) {
                 float value = weighted(x[t][e], d);
-                if (pairs && d < a.turn.dims) {
+                if (turns.pairs && d < a.turn.dims) {
                     int pair;
                     bool is_first;
                     const int other = partner_of(a.turn, d, pair, is_first);
-                    value = turned_once(value, weighted(to_float(from[t * a.stride + other]), other), is_first, turns[t * pairs + pair]);
+                    value = turned_once(value, weighted(to_float(from[t * a.stride + other]), other), is_first, turns.wide[t * turns.pitch + pair]);
                 }
                 x[t][e] = value;
                 largest = fmaxf(largest, counted_magnitude(value));
@@ -409,14 +437,17 @@ __device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const
 // A block of threads: a run of rows after another (those that begin in its `per` rows). The cosines and sines of the run's positions are made
 // once for all heads; then every wave takes heads: keys, values, queries.
 template <typename T, int E, bool PIECES>
-__global__ __launch_bounds__(256) void scaled_append_kernel(AppendArguments a, int per) {
-    extern __shared__ double2 turns[];   // [16][pairs] of queries and keys, then of values
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, waves = blockDim.x / WAVE;
+__global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_append_kernel(AppendArguments a, int per) {
+    extern __shared__ double2 tables[];   // of queries and keys, of values, and of queries in 32 bits
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
     const int window = blockIdx.x * per;
     const bool keeps = a.k_at >= 0;
     uint32_t begins = keeps ? run_begins(a.slots, window, a.n_rows, a.n_slots, lane) : 0xffffffffu;
     const int pairs = a.turn.frequencies ? a.turn.dims / 2 : 0, v_pairs = a.v_turn.frequencies && keeps ? a.v_turn.dims / 2 : 0;
-    double2* const v_turns = turns + BLOCK_TOKENS * pairs;
+    double2* const wide = tables;
+    double2* const v_wide = wide + BLOCK_TOKENS * turn_pitch(pairs);
+    float2* const narrow = reinterpret_cast<float2*>(v_wide + BLOCK_TOKENS * turn_pitch(v_pairs));
+    const TurnTable turns = {wide, narrow, pairs, turn_pitch(pairs)}, v_turns = {v_wide, nullptr, v_pairs, turn_pitch(v_pairs)};
 
     while (begins) {
         const int at = __builtin_ctz(begins);
@@ -424,7 +455,7 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(AppendArguments a, i
         run.first = window + at;
         if (at >= per || run.first >= a.n_rows) return;
         begins &= begins - 1;
-        run.count = min((begins ? __builtin_ctz(begins) : 32) - at, a.n_rows - run.first);   // at most 16
+        run.count = __builtin_amdgcn_readfirstlane(min((begins ? __builtin_ctz(begins) : 32) - at, a.n_rows - run.first));   // at most 16
         const int slot = keeps ? a.slots[run.first] : -1;
         run.kept = slot >= 0 && slot < a.n_slots;
         run.lead = slot & (BLOCK_TOKENS - 1);
@@ -437,19 +468,23 @@ __global__ __launch_bounds__(256) void scaled_append_kernel(AppendArguments a, i
                 const int j = of_value ? i - run.count * pairs : i, n = of_value ? v_pairs : pairs;
                 double c, s;
                 turn_of(a.positions[run.first + j / n], (of_value ? a.v_turn : a.turn).frequencies[j % n], c, s);
-                (of_value ? v_turns : turns)[j] = make_double2(c, s);
+                const int to = (j / n) * turn_pitch(n) + j % n;
+                (of_value ? v_wide : wide)[to] = make_double2(c, s);
+                if (!of_value) narrow[to] = make_float2((float)c, (float)s);
             }
             __syncthreads();
         }
         const int keys = run.kept ? a.n_kv_heads : 0;
         const int queries = a.q_at < 0 ? 0 : PIECES ? a.n_heads : a.n_heads * run.count;
         for (int job = blockIdx.y * waves + wave; job < 2 * keys + queries; job += gridDim.y * waves) {
+            int here = lane;
+            asm volatile("" : "+s"(run.count), "+v"(here));   // (what follows from them is worked out in each job: kept across jobs it takes the registers of half the waves)
             if (job < keys) {
-                if constexpr (PIECES) keys_in_pieces<T, E>(a, run, job, turns, pairs, lane);
-                else keys_by_elements<T, E>(a, run, job, turns, pairs, lane);
-            } else if (job < 2 * keys) append_values<T, E>(a, run, job - keys, v_turns, v_pairs, lane);
-            else if constexpr (PIECES) queries_in_pieces<T, E>(a, run, job - 2 * keys, turns, pairs, lane);
-            else query_by_elements<T, E>(a, run, (job - 2 * keys) / a.n_heads, (job - 2 * keys) % a.n_heads, turns, pairs, lane);
+                if constexpr (PIECES) keys_in_pieces<T, E>(a, run, job, turns, here);
+                else keys_by_elements<T, E>(a, run, job, turns, here);
+            } else if (job < 2 * keys) append_values<T, E>(a, run, job - keys, v_turns, here);
+            else if constexpr (PIECES) queries_in_pieces<T, E>(a, run, job - 2 * keys, turns, here);
+            else query_by_elements<T, E>(a, run, (job - 2 * keys) / a.n_heads, (job - 2 * keys) % a.n_heads, turns, here);
         }
         if (pairs + v_pairs) __syncthreads();
     }
@@ -467,15 +502,15 @@ __device__ __forceinline__ void store_two(T* to, float a, float b) {
 template <typename T>
 __global__ __launch_bounds__(256) void scaled_rows_kernel(const uint8_t* __restrict__ k_codes, const float* __restrict__ k_scales, const uint8_t* __restrict__ v_codes,
                                                           const float* __restrict__ v_scales, const int* __restrict__ slots, long long n_slots, T* __restrict__ k_out,
-                                                          T* __restrict__ v_out, int n_rows, int n_kv_heads, int head_size, int page_shift) {
+                                                          T* __restrict__ v_out, int n_rows, int n_kv_heads, int head_size, int page_shift, int per) {
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    const int window = blockIdx.x * BLOCK_TOKENS, head = blockIdx.y * 4 + wave;
+    const int window = blockIdx.x * per, head = blockIdx.y * 4 + wave;
     if (head >= n_kv_heads) return;
     const size_t row_size = (size_t)n_kv_heads * head_size;
     uint32_t begins = run_begins(slots, window, n_rows, n_slots, lane);
     while (begins) {
         const int at = __builtin_ctz(begins), first = window + at;
-        if (at >= BLOCK_TOKENS || first >= n_rows) return;
+        if (at >= per || first >= n_rows) return;
         begins &= begins - 1;
         const int count = min((begins ? __builtin_ctz(begins) : 32) - at, n_rows - first);
         const int slot = slots[first];
@@ -563,10 +598,9 @@ MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, in
     const int per = n_rows >= 256 && k_at >= 0 ? BLOCK_TOKENS : 1;
     const int blocks = ceil_div(n_rows, per);
     const int jobs = (k_at >= 0 ? 2 * n_kv_heads : 0) + (q_at < 0 ? 0 : on_pieces ? n_heads : n_heads * per);
-    int shares = 1;
-    while (blocks * shares < APPEND_BLOCKS && shares * 4 < jobs) shares *= 2;
+    const int shares = std::max(1, std::min(ceil_div(APPEND_BLOCKS, blocks), jobs / 4));
     const dim3 grid(blocks, shares);
-    const size_t lds = (size_t)BLOCK_TOKENS * (rot_dims / 2 + v_rot_dims / 2) * sizeof(double2);
+    const size_t lds = (size_t)BLOCK_TOKENS * (turn_pitch(rot_dims / 2) * (sizeof(double2) + sizeof(float2)) + turn_pitch(v_rot_dims / 2) * sizeof(double2));
     mllm_count_kernel(MLLM_K_SCALED_APPEND);
 #define APPEND_CASE(T, E)                                                              \
     if (on_pieces) scaled_append_kernel<T, E, true><<<grid, 256, lds, stream>>>(a, per); \
@@ -591,14 +625,16 @@ MLLM_API int mllm_scaled_rows(const void* k_codes, const float* k_scales, const 
     MLLM_REQUIRE(page_size >= BLOCK_TOKENS && (page_size & (page_size - 1)) == 0, "scaled_rows: page size %d is no power of two of at least %d", page_size, BLOCK_TOKENS);
     MLLM_REQUIRE(dtype == MLLM_F32 || dtype == MLLM_BF16, "scaled_rows: unknown dtype %d", dtype);
     if (n_rows == 0) return 0;
-    const dim3 grid(ceil_div(n_rows, BLOCK_TOKENS), ceil_div(n_kv_heads, 4));
+    // few rows: a block of threads for every two (most of which begin no run and have nothing to do), so that runs do not wait for each other
+    const int per = (long long)n_rows * n_kv_heads >= 16384 ? BLOCK_TOKENS : 2;
+    const dim3 grid(ceil_div(n_rows, per), ceil_div(n_kv_heads, 4));
     const long long n_slots = (long long)num_pages * page_size;
     mllm_count_kernel(MLLM_K_SCALED_ROWS);
     if (dtype == MLLM_F32)
         scaled_rows_kernel<float><<<grid, 256, 0, stream>>>((const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales, slots, n_slots, (float*)k_out, (float*)v_out,
-                                                            n_rows, n_kv_heads, head_size, shift_of(page_size));
+                                                            n_rows, n_kv_heads, head_size, shift_of(page_size), per);
     else
         scaled_rows_kernel<bf16_t><<<grid, 256, 0, stream>>>((const uint8_t*)k_codes, k_scales, (const uint8_t*)v_codes, v_scales, slots, n_slots, (bf16_t*)k_out, (bf16_t*)v_out,
-                                                             n_rows, n_kv_heads, head_size, shift_of(page_size));
+                                                             n_rows, n_kv_heads, head_size, shift_of(page_size), per);
     return mllm_check_launch("scaled_rows");
 }

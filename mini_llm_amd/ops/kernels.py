@@ -1639,16 +1639,21 @@ SCALED_SHORT = 8            # portions up to so many tokens go row by row
 def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int, wide: bool = False) -> tuple[int, int, int]:
     """(waves a block, tiles a run, runs) for the rows kernel over pages of 8 bits: ``blocks`` (row, head group) pairs, each with up to ``tiles`` tiles of
     keys, ``columns`` heads of ``head_size`` a block; ``wide``: queries in 32-bit."""
-    most = (8 if wide else 16) if head_size <= 64 else 8 if head_size <= 128 else 4
-    while most > 1 and most * columns * (head_size + 4) * 4 > 65536:
+    most = (8 if wide else 16) if head_size <= 64 else 8 if head_size <= 128 else 4   # (what the registers leave)
+    while most > 1 and most * columns * (head_size + 4) * 4 > 65536:   # and what the LDS holds of their results
         most //= 2
-    run = tiles
-    while run > most and blocks * -(-tiles // run) < 512:
-        run = -(-run // 2)
+    # Rows of few tiles and launches of many blocks are not cut: putting runs together is another launch. us of 12 blocks of 16 tiles in 1 / 4 / 8 runs 7.5 / 9.0 /
+    # 9.0; of 200 of 15 (32-bit) in 1 / 3 / 5 11.1 / 14.3 / 13.6; of 768 of 63 in 1 / 3 / 5 60 / 64 / 65. Others are cut until there are two blocks for each of
+    # 256 compute units, into at most about sqrt(tiles) runs: of 12 of 63 in 3 / 5 / 9 / 21 11.0 / 9.9 / 9.9 / 10.4; of 8 of 469 (heads of 128) in 5 / 9 / 17 / 34 / 59
+    # 33 / 24 / 22 / 28 / 32; of 96 of 63 (32-bit) in 1 / 5 / 9 / 21 22.2 / 18.6 / 19.4 / 19.4; of 128 of 480 in 2 / 4 / 8 150 / 150 / 156.
+    runs = 1 if tiles <= 2 * most else max(1, min(512 // max(blocks, 1), round(0.8 * tiles**0.5)))
+    run = -(-tiles // runs)
+    runs = -(-tiles // run)
+    # Waves: as many as have a tile, up to 12 a compute unit (768 blocks of 16 tiles with 2 / 4 / 8 waves 15.5 / 15.3 / 17.3; 512 14.3 / 12.4 / 13.0).
     waves = 1
-    while waves < most and waves < run and (blocks * -(-tiles // run)) * waves < 4096:
+    while waves < most and waves < run and 2 * waves * blocks * runs <= 3072:
         waves *= 2
-    return waves, run, -(-tiles // run)
+    return waves, run, runs
 
 
 def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_tables, n_heads, n_kv_heads, head_size, scale, window, max_q_len, max_len, q_starts, context_lens, out,
