@@ -200,9 +200,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention
         float meeting[WAVES][ROWS][PITCH];
     } lds;
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-    const int request = blockIdx.z, head = blockIdx.y, head_size = a.planes.head_size;
+    const int request = blockIdx.z, head = blockIdx.x, head_size = a.planes.head_size;
     const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
-    const int row0 = (gridDim.x - 1 - blockIdx.x) * ROWS;
+    const int row0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
     const int context = a.context_lens[request];
     if (row0 >= q_len || context < 0 || q_first < 0) return;   // (a negative context: a padding request, whose rows are nobody's)
     const int kv_head = head / (a.n_heads / a.planes.n_kv_heads);
@@ -352,12 +352,12 @@ MLLM_API int mllm_scaled_attention_tiles(const void* q, long long q_stride, cons
                                          n_kv_heads, head_size, page_size, window, scale, dtype, softcap, sinks, chunk, keep, wide_out);
     a.q_starts = q_starts, a.context_lens = context_lens;
     if (int status = refuse_attend("scaled_attention_tiles", a, page_size, dtype)) return status;
-    MLLM_REQUIRE(n_requests <= 65535 && n_heads <= 65535, "scaled_attention_tiles: too many requests or heads for one launch");
+    MLLM_REQUIRE(n_requests <= 65535 && max_q_len <= 65535 * 16, "scaled_attention_tiles: too many requests or rows for one launch");
     if (n_rows == 0 || max_q_len <= 0) return 0;
     mllm_count_kernel(MLLM_K_SCALED_ATTENTION_TILES);
 #define TILES_CASE(T, HD, CT)                                                                                   \
     {                                                                                                           \
-        const dim3 grid(ceil_div(max_q_len, 16 * CT), n_heads, n_requests);                                     \
+        const dim3 grid(n_heads, ceil_div(max_q_len, 16 * CT), n_requests);                                     \
         if (page_size >= TILE_KEYS) scaled_tiles_attention_kernel<T, HD, CT, true><<<grid, 256, 0, stream>>>(a); \
         else scaled_tiles_attention_kernel<T, HD, CT, false><<<grid, 256, 0, stream>>>(a);                       \
     }
