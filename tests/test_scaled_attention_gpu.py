@@ -119,6 +119,23 @@ def test_masks_caps_and_sinks(dtype, size, options):
     check(batch, batch.run(**given), **options)                                    # single rows as portions
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,size,page", [("bf16", 40, 2, 64, 64), ("bf16", 48, 4, 64, 16), ("bf16", 40, 1, 128, 64), ("bf16", 48, 2, 112, 32),
+                                                            ("f32", 40, 2, 64, 64), ("f32", 48, 4, 48, 16)])
+@pytest.mark.parametrize("options", [{}, dict(window=70, keep_first=5, softcap=4.0)], ids=["whole", "window"])
+def test_many_blocks_take_more_rows_each(dtype, heads, kv_heads, size, page, options):
+    """Enough blocks (320 of the larger tiles of rows) for the form that launches of fewer do not take; with numbers that are none in masked places
+    and in one that some rows of a tile see."""
+    batch = Batch(dtype, heads, kv_heads, size, page, [0, 37], [520, 61], seed=size)
+    for plane in batch.planes:
+        plane.codes[batch.unused] = torch.nan
+    batch.planes[1].codes[int(batch.tables[0, 300 // page]), 0, 300 % page, 3] = torch.nan
+    got = batch.run(**options).double().cpu()
+    want = batch.want(**options)
+    lost = torch.isnan(want)
+    assert bool(lost.any()) and torch.equal(torch.isnan(got), lost)
+    close(torch.where(lost, 0.0, got), torch.where(lost, 0.0, want), batch)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_short_portions_go_row_by_row(dtype):
     batch = Batch(dtype, 4, 2, 64, 64, [0, 100, 63, 5], [8, 3, 2, 1], seed=3)
