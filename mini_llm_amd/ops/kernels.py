@@ -1492,20 +1492,23 @@ class ScaledPages:
     dtype = E4M3
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
-        _require(isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor), "codes and scales are tensors")
-        if codes.dtype != E4M3 or scales.dtype != torch.float32:
-            raise OperandError(f"codes are {E4M3} and scales float32, not {codes.dtype} and {scales.dtype}")
+        if not (isinstance(codes, torch.Tensor) and isinstance(scales, torch.Tensor) and codes.dtype == E4M3 and scales.dtype == torch.float32):
+            raise OperandError(f"codes are a tensor of {E4M3} and scales one of float32")
         self.device_index = codes.get_device()   # -1: not on a GPU
-        _require(codes.is_contiguous() and scales.is_contiguous() and scales.get_device() == self.device_index, "codes and scales are contiguous and lie on one device")
-        of_codes, of_scales = tuple(codes.shape), tuple(scales.shape)
-        self.is_keys = len(of_codes) == 6
-        _require(len(of_codes) in (5, 6) and of_codes[-1] == SCALE_BLOCK and of_codes[4] == SCALE_BLOCK, "codes have neither the shape of keys nor that of values")
-        _require(of_scales == of_codes[:3], "one scale a block")
-        page_size, head_size = of_codes[2] * SCALE_BLOCK, of_codes[3] * (16 if self.is_keys else 1)
-        if not (of_codes[0] > 0 and of_codes[1] > 0 and page_size >= SCALE_BLOCK and page_size & (page_size - 1) == 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD):
+        if not (codes.is_contiguous() and scales.is_contiguous() and scales.get_device() == self.device_index):
+            raise OperandError("codes and scales are contiguous and lie on one device")
+        of_codes = codes.shape
+        keys = self.is_keys = len(of_codes) == 6
+        if not ((keys or len(of_codes) == 5) and of_codes[-1] == SCALE_BLOCK and of_codes[4] == SCALE_BLOCK):
+            raise OperandError("codes have neither the shape of keys nor that of values")
+        if scales.shape != of_codes[:3]:
+            raise OperandError("one scale a block")
+        num_pages, n_kv_heads, blocks = of_codes[0], of_codes[1], of_codes[2]
+        page_size, head_size = blocks * SCALE_BLOCK, of_codes[3] * 16 if keys else of_codes[3]
+        if not (num_pages > 0 and n_kv_heads > 0 and blocks > 0 and blocks & (blocks - 1) == 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD):
             raise OperandError(f"pages of {page_size} tokens (a power of two of at least {SCALE_BLOCK}) for heads of {head_size} (a multiple of 16 up to {SCALED_MAX_HEAD})")
-        self.codes, self.scales, self.on_gpu = codes, scales, self.device_index >= 0 and codes.is_cuda
-        self.shape, self.addresses = (of_codes[0], of_codes[1], page_size, head_size), (codes.data_ptr(), scales.data_ptr())
+        self.codes, self.scales, self.on_gpu = codes, scales, self.device_index >= 0
+        self.shape, self.addresses = (num_pages, n_kv_heads, page_size, head_size), (codes.data_ptr(), scales.data_ptr())
 
     @property
     def device(self):
@@ -1554,11 +1557,16 @@ def _floats(t, name: str, count: int, here: int):
     return t.data_ptr()
 
 
-def _strided_rows(t, name: str, width: int, here: int) -> None:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.shape[1] == width and (t.stride(1) == 1 or width == 1)):
+def _strided_rows(t, name: str, width: int, here: int) -> int:
+    """Rows from one to the next of a 2-D tensor with ``width`` contiguous columns on the current device."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.shape[1] == width):
         raise OperandError(f"{name} must be 2-D on the GPU with {width} contiguous columns")
-    _require(t.stride(0) >= width or t.shape[0] <= 1, f"{name}'s rows overlap")
-    _require(t.get_device() == here, f"{name} lies on another device than the current one")
+    stride, across = t.stride()
+    if not ((across == 1 or width == 1) and (stride >= width or t.shape[0] <= 1)):
+        raise OperandError(f"{name} must have {width} contiguous columns, and rows that do not overlap")
+    if t.get_device() != here:
+        raise OperandError(f"{name} lies on another device than the current one")
+    return max(stride, width)
 
 
 def _rotation(frequencies, dims: int, most: int, pairing: str, name: str, here: int):
@@ -1611,7 +1619,7 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     slot_at = _ints(slots, "slots", n, here) if keeps else None
     _require(num_pages * page_size <= 2**31, "the pages hold more tokens than a slot can name")
     out_dtype = out_dtype or rows.dtype
-    q = torch.empty((n, n_heads * head_size), dtype=out_dtype, device=rows.device) if makes else None
+    q = rows.new_empty((n, n_heads * head_size), dtype=out_dtype) if makes else None
     check(library().mllm_scaled_append(rows.data_ptr(), stride, q_at if makes else -1, k_at if keeps else -1, v_at if keeps else -1, q_gain, k_gain, eps, bool(unit), frequencies,
                                        rot_dims, pairing == "neighbours", v_frequencies, v_rot_dims, v_pairing == "neighbours", position_at, slot_at, _ptr(q), *k_pages.addresses,
                                        *v_pages.addresses, num_pages, n, n_heads, n_kv_heads, dim, vdim, head_size, page_size, _code(rows.dtype), _code(out_dtype), _stream()))
@@ -1664,7 +1672,7 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
     num_pages, _, page_size, _ = k_pages.shape
     _require(n_heads > 0 and n_heads % n_kv_heads == 0, f"{n_heads} heads do not divide into {n_kv_heads} key/value heads")
     width, group = n_heads * head_size, n_heads // n_kv_heads
-    _strided_rows(q, "q", width, here)
+    stride = _strided_rows(q, "q", width, here)
     code = _code(q.dtype)
     n = q.shape[0]
     if not (isinstance(block_tables, torch.Tensor) and block_tables.dtype == torch.int32 and block_tables.dim() == 2 and block_tables.get_device() == here and block_tables.is_contiguous()):
@@ -1679,16 +1687,16 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
     sink_at = _floats(sinks, "sinks", n_heads, here)
     out_dtype = torch.float32 if wide_out else q.dtype
     if out is None:
-        out = torch.empty((n, width), dtype=out_dtype, device=q.device)
+        out, out_stride = q.new_empty((n, width), dtype=out_dtype), width
     else:
-        _strided_rows(out, "out", width, here)
+        out_stride = _strided_rows(out, "out", width, here)
         _require(out.dtype == out_dtype and out.shape[0] == n, "out has the wrong shape or type")
     request_at, position_at = _ints(token_request, "token_request", n, here), _ints(positions, "positions", n, here)
     lib = library()
     if n == 0:
         return out
     table_at = block_tables.data_ptr()
-    given = (q.data_ptr(), q.stride(0), *k_pages.addresses, *v_pages.addresses)
+    given = (q.data_ptr(), stride, *k_pages.addresses, *v_pages.addresses)
 
     def rows_alone(count, into, packed):
         reach = max_blocks * page_size
@@ -1698,7 +1706,7 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
             tiles = max(1, min(tiles, -(-int(max_len) // SCALED_TILE)))
         waves, run, runs = scaled_cut(count * n_kv_heads * -(-group // 16), tiles, head_size, min(16, group), code == F32)
         parts = torch.empty((count, n_heads, runs, head_size + 2), dtype=torch.float32, device=q.device) if runs > 1 else None
-        check(lib.mllm_scaled_attention_rows(*given, into.data_ptr(), width if packed else into.stride(0), request_at, position_at, table_at, max_blocks, n_tables, num_pages, count,
+        check(lib.mllm_scaled_attention_rows(*given, into.data_ptr(), width if packed else out_stride, request_at, position_at, table_at, max_blocks, n_tables, num_pages, count,
                                              n_heads, n_kv_heads, head_size, page_size, window, scale, code, softcap, sink_at, chunk, keep, wide_out, packed, waves, run, runs,
                                              _ptr(parts), _stream()))
 
@@ -1718,7 +1726,7 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
         _require(0 < short_requests < n_requests, "short_requests does not cut the batch in two")
         rows_alone(int(short_rows), out, False)
         skipped = int(short_requests)
-    check(lib.mllm_scaled_attention_tiles(*given, out.data_ptr(), out.stride(0), start_at + 4 * skipped, context_at + 4 * skipped, table_at + 4 * skipped * max_blocks, max_blocks,
+    check(lib.mllm_scaled_attention_tiles(*given, out.data_ptr(), out_stride, start_at + 4 * skipped, context_at + 4 * skipped, table_at + 4 * skipped * max_blocks, max_blocks,
                                           n_requests - skipped, num_pages, n, int(max_q_len), n_heads, n_kv_heads, head_size, page_size, window, scale, code, softcap, sink_at, chunk,
                                           keep, wide_out, _stream()))
     return out
