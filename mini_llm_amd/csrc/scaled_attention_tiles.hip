@@ -5,6 +5,9 @@
 
 namespace {
 
+constexpr int MOST_ROWS = 65535 * 16;                   // of a portion in one launch
+constexpr int MOST_REACH = 2147483647 - 2 * MOST_ROWS;   // positions, the rows of a block that a portion does not have among them, are numbers of 32 bits
+
 // Portions of prompts: a block per (request, head, tile of 16 CT rows), whose waves hold all those rows and take the tiles of keys in turn,
 // each with statistics of its own, and meet in LDS. Tiles with the most keys come first.
 template <typename T, int HD, int CT, bool WHOLE>
@@ -22,10 +25,10 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention
     const int request = blockIdx.z, head = blockIdx.x, head_size = a.planes.head_size;
     const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
     const int row0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
-    const int context = a.context_lens[request];
+    const int reach = (int)min((long long)a.max_blocks << a.planes.page_shift, (long long)MOST_REACH) - 1;
+    const int context = min(a.context_lens[request], reach);
     if (row0 >= q_len || context < 0 || q_first < 0) return;   // (a negative context: a padding request, whose rows are nobody's)
     const int kv_head = head / (a.n_heads / a.planes.n_kv_heads);
-    const int reach = (int)min((long long)a.max_blocks << a.planes.page_shift, 2147483647LL) - 1;
     const int position0 = min(context + row0, reach), position1 = min(context + min(row0 + ROWS, q_len) - 1, reach);
 
     Sweep sweep;
@@ -92,7 +95,7 @@ MLLM_API int mllm_scaled_attention_tiles(const void* q, long long q_stride, cons
                                          n_kv_heads, head_size, page_size, window, scale, dtype, softcap, sinks, chunk, keep, wide_out);
     a.q_starts = q_starts, a.context_lens = context_lens;
     if (int status = refuse_attend("scaled_attention_tiles", a, page_size, dtype)) return status;
-    MLLM_REQUIRE(n_requests <= 65535 && max_q_len <= 65535 * 16, "scaled_attention_tiles: too many requests or rows for one launch");
+    MLLM_REQUIRE(n_requests <= 65535 && max_q_len <= MOST_ROWS, "scaled_attention_tiles: too many requests or rows for one launch");
     if (n_rows == 0 || max_q_len <= 0) return 0;
     mllm_count_kernel(MLLM_K_SCALED_ATTENTION_TILES);
     // Rows a block: as many as the registers hold the sums of (a key is converted once for all of them), or half as many where that leaves fewer

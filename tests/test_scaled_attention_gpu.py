@@ -327,3 +327,41 @@ def test_a_layer_step_captured_and_replayed(dtype):
         assert torch.equal(out, want), step
     for a, b in zip(eager, captured):
         assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+
+
+@pytest.mark.parametrize("news", [[1, 1], [40, 70]], ids=["rows", "portions"])
+def test_pages_beyond_offsets_of_32_bits(news):
+    """The same requests in the first pages and in the last of a cache whose planes are larger than 2^32 bytes."""
+    K, page, heads, kv_heads, size, num_pages = kernels(), 64, 16, 8, 128, 68000
+    k_pages, v_pages = K.scaled_pages(num_pages, kv_heads, page, size, DEVICE)
+    assert k_pages.codes.numel() > 2**32
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEVICE)
+    contexts, total = [200, 30], sum(news)
+    g = torch.Generator().manual_seed(12)
+    stored = [torch.randn((c + n, 2 * kv_heads * size), generator=g).to(DEVICE) for c, n in zip(contexts, news)]
+    q = torch.randn((total, heads * size), generator=g).bfloat16().to(DEVICE)
+    positions = ints([c + i for c, n in zip(contexts, news) for i in range(n)])
+    owner = ints([r for r, n in enumerate(news) for _ in range(n)])
+    results = []
+    for first in (0, num_pages - 16):
+        tables = torch.arange(first, first + 16, dtype=torch.int32, device=DEVICE).view(2, 8).flip(0).contiguous()
+        for rows, table in zip(stored, tables):
+            at = torch.arange(rows.shape[0], device=DEVICE)
+            K.scaled_append(rows, None, 0, kv_heads * size, k_pages, v_pages, (table[at // page] * page + (at % page).int()).int(), at.int(), heads, kv_heads, size, size)
+        results.append(K.paged_attention(q, k_pages, v_pages, owner, positions, tables, heads, kv_heads, size, size**-0.5, max_q_len=max(news), max_len=512,
+                                         q_starts=ints([0, news[0], total]), context_lens=ints(contexts)))
+        read = K.scaled_rows(k_pages, v_pages, (tables[0, :1] * page).contiguous())[1]
+        assert bool(((read.double() - stored[0][0, kv_heads * size :].view(kv_heads, size).double()).abs() <= stored[0].abs().max() * 2.0**-4).all())
+    assert bool(results[0].any()) and torch.equal(results[0], results[1])
+
+
+def test_a_context_at_the_end_of_all_numbers_stays_in_its_table():
+    """A length that no table reaches counts as the table's last position: nothing is read behind it (its rows' results are nobody's)."""
+    K = kernels()
+    k_pages, v_pages = K.scaled_pages(4, 2, 64, 64, DEVICE)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEVICE)
+    n = 30
+    q = torch.randn((n, 128), device=DEVICE)
+    out = K.paged_attention(q, k_pages, v_pages, ints([0] * n), ints(list(range(n))), ints([[0, 1, 2, 3]]), 2, 2, 64, 0.125, max_q_len=n, max_len=256, q_starts=ints([0, n]),
+                            context_lens=ints([2**31 - 3]))
+    assert out.shape == (n, 128) and not bool(out.any())   # (the pages hold zeros)
