@@ -442,7 +442,8 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
     const int window = blockIdx.x * per;
     const bool keeps = a.k_at >= 0;
-    uint32_t begins = keeps ? run_begins(a.slots, window, a.n_rows, a.n_slots, lane) : 0xffffffffu;
+    // (queries alone have no blocks: any rows are a run)
+    uint32_t begins = keeps ? run_begins(a.slots, window, a.n_rows, a.n_slots, lane) : per == 1 ? 0xffffffffu : 0x00010001u;
     const int pairs = a.turn.frequencies ? a.turn.dims / 2 : 0, v_pairs = a.v_turn.frequencies && keeps ? a.v_turn.dims / 2 : 0;
     double2* const wide = tables;
     double2* const v_wide = wide + BLOCK_TOKENS * turn_pitch(pairs);
@@ -594,8 +595,9 @@ MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, in
     const int size = dtype == MLLM_F32 ? 4 : 2;
     const bool on_pieces = (uintptr_t)rows % 16 == 0 && stride * size % 16 == 0 && dim % 16 == 0 && rot_dims % 16 == 0 && (q_at < 0 || (q_at * size % 16 == 0 && (uintptr_t)q_out % 16 == 0)) &&
                            (k_at < 0 || k_at * size % 16 == 0);
-    // many rows: 16 to a block of threads, which finds the runs among them; few: a block each, so that each is under way at once
-    const int per = n_rows >= 256 && k_at >= 0 ? BLOCK_TOKENS : 1;
+    // many rows: 16 to a block of threads, which finds the runs among them; few: a block each, so that each is under way at once. Queries alone, 32 heads of 128 turned, us with
+    // one row / 16 a block: 32 rows 5.5 / 6.4, 64 6.0 / 6.4, 128 9.4 / 6.5, 8,192 202 / 32.6.
+    const int per = n_rows >= (k_at >= 0 ? 256 : 96) ? BLOCK_TOKENS : 1;
     const int blocks = ceil_div(n_rows, per);
     const int jobs = (k_at >= 0 ? 2 * n_kv_heads : 0) + (q_at < 0 ? 0 : on_pieces ? n_heads : n_heads * per);
     const int shares = std::max(1, std::min(ceil_div(APPEND_BLOCKS, blocks), jobs / 4));

@@ -216,3 +216,44 @@ def test_token_by_token_and_at_once_hold_the_same_where_the_scale_does_not_grow(
         K.scaled_append(rows[r : r + 1], None, 0, heads * size, *by_one, ints([r]), ints([0]), heads, heads, size, size)
     for a, b in zip(once, by_one):
         assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 40])
+def test_many_queries_alone(dtype, dim):
+    """Rows of queries alone are taken sixteen at a time, the last of them fewer."""
+    K, heads, n = kernels(), 3, 16 * 16 + 5
+    g = torch.Generator().manual_seed(4)
+    rows = torch.randn((n, heads * dim), generator=g).to(TYPES[dtype])
+    positions = torch.randint(0, 5000, (n,), generator=g, dtype=torch.int32)
+    f = 10000.0 ** (-torch.arange(8, dtype=torch.float64) / 8)
+    k_pages, v_pages = K.scaled_pages(1, 1, 16, 64, DEVICE)
+    q = K.scaled_append(rows.to(DEVICE), 0, None, None, k_pages, v_pages, None, positions.to(DEVICE), heads, 1, dim, dim, frequencies=f.to(DEVICE), rot_dims=16)
+    want = turned(rows.double().view(n, heads, dim), positions, f, 16, "half")
+    got = q.cpu().double().view(n, heads, 64)
+    # two products and a sum in 32-bit (cosine and sine rounded to it), and the rounding to the type
+    assert bool(((got[..., :dim] - want).abs() <= torch.finfo(TYPES[dtype]).eps / 2 * want.abs() + 2.0**-22 * rows.double().abs().amax() * 2).all())
+    assert not bool(got[..., dim:].any())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [256, 250])
+def test_the_widest_heads_turned_whole(dtype, dim):
+    """Tables of the cosines of 128 pairs, of keys and of values: more memory of a block than any other call takes."""
+    K, n = kernels(), 40
+    slots, planes = prepared([5], [n], 32, 2, 256, 8)
+    g = torch.Generator().manual_seed(9)
+    rows = torch.randn((n, 5 * dim), generator=g).to(TYPES[dtype])
+    positions = torch.randint(0, 5000, (n,), generator=g, dtype=torch.int32)
+    f = 10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2))
+    k_pages, v_pages = pages_of(planes)
+    q = K.scaled_append(rows.to(DEVICE), 0, dim, 3 * dim, k_pages, v_pages, torch.tensor(slots, dtype=torch.int32, device=DEVICE), positions.to(DEVICE), 1, 2, dim, dim,
+                        frequencies=f.to(DEVICE), rot_dims=dim, v_frequencies=f.to(DEVICE), v_rot_dims=dim, v_pairing="neighbours")
+    wide = rows.double()
+    want = turned(wide[:, :dim].view(n, 1, dim), positions, f, dim, "half")
+    got = q.cpu().double().view(n, 1, 256)[..., :dim]
+    assert bool(((got - want).abs() <= torch.finfo(TYPES[dtype]).eps / 2 * want.abs() + 2.0**-22 * rows.double().abs().amax() * 2).all())
+    planes[0].append(turned(wide[:, dim : 3 * dim].reshape(n, 2, dim), positions, f, dim, "half"), slots)
+    planes[1].append(turned(wide[:, 3 * dim :].reshape(n, 2, dim), positions, f, dim, "neighbours"), slots)
+    for got, plane in zip(held_by(k_pages, v_pages), planes):
+        same(got, plane.held())
