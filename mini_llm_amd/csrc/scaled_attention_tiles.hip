@@ -8,20 +8,21 @@ namespace {
 constexpr int MOST_ROWS = 65535 * 16;                   // of a portion in one launch
 constexpr int MOST_REACH = 2147483647 - 2 * MOST_ROWS;   // positions, the rows of a block that a portion does not have among them, are numbers of 32 bits
 
-// Portions of prompts: a block per (request, head, tile of 16 CT rows), whose waves hold all those rows and take the tiles of keys in turn,
-// each with statistics of its own, and meet in LDS. Tiles with the most keys come first.
-template <typename T, int HD, int CT, bool WHOLE>
+// Portions of prompts: a block per (request, head, tile of rows). SPLITS of its four waves take the tiles of keys in turn, each with statistics of
+// its own, and meet in LDS; with two, the other two do the same for 16 CT rows more, at the same time, so that half of what they read comes from
+// the compute unit's own cache. Tiles with the most keys of all heads come first.
+template <typename T, int HD, int CT, int SPLITS, bool WHOLE>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention_kernel(AttendArguments a) {
     constexpr bool WIDE = sizeof(T) == 4;
     typedef ScaledSweep<HD, CT, WIDE, true, WHOLE> Sweep;
-    constexpr int ROWS = 16 * CT, WAVES = 4;
+    constexpr int WAVES = 4, GROUPS = WAVES / SPLITS, WAVE_ROWS = 16 * CT, ROWS = GROUPS * WAVE_ROWS;
     // the queries' operands while keys are walked; then what the waves hold, row by row
     constexpr int PITCH = HD + 4;
     __shared__ union {
-        bf16x8 queries[Sweep::Q_PIECES];
-        float meeting[WAVES][ROWS][PITCH];
+        bf16x8 queries[GROUPS][Sweep::Q_PIECES];
+        float meeting[WAVES][WAVE_ROWS][PITCH];
     } lds;
-    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = wave % GROUPS, split = wave / GROUPS;
     const int request = blockIdx.z, head = blockIdx.x, head_size = a.planes.head_size;
     const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
     const int row0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
@@ -29,24 +30,27 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention
     const int context = min(a.context_lens[request], reach);
     if (row0 >= q_len || context < 0 || q_first < 0) return;   // (a negative context: a padding request, whose rows are nobody's)
     const int kv_head = head / (a.n_heads / a.planes.n_kv_heads);
-    const int position0 = min(context + row0, reach), position1 = min(context + min(row0 + ROWS, q_len) - 1, reach);
+    const int own0 = row0 + group * WAVE_ROWS;   // the wave's first row, if the portion has it
+    const int position0 = min(context + own0, reach), position1 = min(context + min(own0 + WAVE_ROWS, q_len) - 1, reach);
 
     Sweep sweep;
     sweep.init(head_size, lane);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-        const int local = row0 + 16 * ct + lane % 16;
+        const int local = own0 + 16 * ct + lane % 16;
         const bool valid = local < q_len;
-        if (ct % WAVES == wave) {
+        if (ct % SPLITS == split) {
             sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
-            sweep.share_query(ct, lds.queries, lane);
+            sweep.share_query(ct, lds.queries[group], lane);
         }
     }
-    sweep.q_shared = lds.queries;
+    sweep.q_shared = lds.queries[group];
     __syncthreads();
-    const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
-    sweep.tiles(range, wave, WAVES, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale,
-                {context + row0 + lane % 16, position1, a.window, a.chunk, a.keep}, scaled_first_key(position1, a.window, a.chunk), position0, lane);
+    if (GROUPS == 1 || own0 < q_len) {
+        const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
+        sweep.tiles(range, split, SPLITS, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale,
+                    {context + own0 + lane % 16, position1, a.window, a.chunk, a.keep}, scaled_first_key(position1, a.window, a.chunk), position0, lane);
+    }
 
     __syncthreads();   // (all waves are through with the queries)
 #pragma unroll
@@ -66,16 +70,18 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention
     for (int i = threadIdx.x; i < ROWS * fours; i += blockDim.x) {
         const int row = i / fours, d = 4 * (i % fours);
         if (row0 + row >= q_len) break;
+        const int of_group = GROUPS == 1 ? 0 : row / WAVE_ROWS, at = GROUPS == 1 ? row : row % WAVE_ROWS;
         float top = NO_SCORE;
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) top = fmaxf(top, lds.meeting[w][row][HD]);
+        for (int w = 0; w < SPLITS; w++) top = fmaxf(top, lds.meeting[w * GROUPS + of_group][at][HD]);
         float total = a.sinks ? weight_of<WIDE>(a.sinks[head] * a.sink_factor - top) : 0.0f;
         f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const float factor = weight_of<WIDE>(lds.meeting[w][row][HD] - top);
-            total += lds.meeting[w][row][HD + 1] * factor;
-            const f32x4 theirs = *reinterpret_cast<const f32x4*>(&lds.meeting[w][row][d]);
+        for (int w = 0; w < SPLITS; w++) {
+            const float* const part = lds.meeting[w * GROUPS + of_group][at];
+            const float factor = weight_of<WIDE>(part[HD] - top);
+            total += part[HD + 1] * factor;
+            const f32x4 theirs = *reinterpret_cast<const f32x4*>(part + d);
 #pragma unroll
             for (int e = 0; e < 4; e++) value[e] += theirs[e] * factor;
         }
@@ -104,24 +110,29 @@ MLLM_API int mllm_scaled_attention_tiles(const void* q, long long q_stride, cons
     // 16 heads of 128, 512 rows (256) 9.7 / 8.3, 2,048 (1,024) 35.4 / 47.0; in 32-bit 12 heads of 64, 512 rows 10.5 / 8.7, 2,048 (768) 38.7 / 38.3.
     const int whole = dtype == MLLM_F32 ? (head_size <= 64 ? 2 : 1) : head_size <= 64 ? 4 : head_size <= 128 ? 2 : 1;
     const long long by_rows = n_rows / (16 * whole) + n_requests, by_longest = (long long)n_requests * ceil_div(max_q_len, 16 * whole);
-    const bool half = n_heads * std::min(by_rows, by_longest) < 320;
-#define TILES_CASE(T, HD, CT)                                                                                   \
-    {                                                                                                           \
-        const dim3 grid(n_heads, ceil_div(max_q_len, 16 * CT), n_requests);                                     \
-        if (page_size >= TILE_KEYS) scaled_tiles_attention_kernel<T, HD, CT, true><<<grid, 256, 0, stream>>>(a); \
-        else scaled_tiles_attention_kernel<T, HD, CT, false><<<grid, 256, 0, stream>>>(a);                       \
+    const long long blocks = n_heads * std::min(by_rows, by_longest);
+    const bool half = blocks < 320;
+    // Heads of 65 to 128, twice the rows a block (half the waves on each) where there are blocks in plenty: us with 32 / 64 rows, 16 heads of 128 on 2,048 rows (1,024 / 512
+    // blocks) 35.8 / 36.4, 32 on 1,024 behind 3,072 keys (1,024 / 512) 83.9 / 82.8, 16 on 8,192 (4,096 / 2,048) 299 / 285. (Of 64, on 8,192: 144 / 151.)
+    const bool twice = blocks >= 2048;
+#define TILES_CASE(T, HD, CT, S)                                                                                   \
+    {                                                                                                              \
+        const dim3 grid(n_heads, ceil_div(max_q_len, 16 * CT * (4 / S)), n_requests);                              \
+        if (page_size >= TILE_KEYS) scaled_tiles_attention_kernel<T, HD, CT, S, true><<<grid, 256, 0, stream>>>(a); \
+        else scaled_tiles_attention_kernel<T, HD, CT, S, false><<<grid, 256, 0, stream>>>(a);                       \
     }
     if (dtype == MLLM_F32) {
-        if (head_size > 128) TILES_CASE(float, 256, 1)
-        else if (head_size > 64) TILES_CASE(float, 128, 1)
-        else if (half) TILES_CASE(float, 64, 1)
-        else TILES_CASE(float, 64, 2)
-    } else if (head_size > 128) TILES_CASE(bf16_t, 256, 1)
+        if (head_size > 128) TILES_CASE(float, 256, 1, 4)
+        else if (head_size > 64) TILES_CASE(float, 128, 1, 4)
+        else if (half) TILES_CASE(float, 64, 1, 4)
+        else TILES_CASE(float, 64, 2, 4)
+    } else if (head_size > 128) TILES_CASE(bf16_t, 256, 1, 4)
     else if (head_size > 64) {
-        if (half) TILES_CASE(bf16_t, 128, 1)
-        else TILES_CASE(bf16_t, 128, 2)
-    } else if (half) TILES_CASE(bf16_t, 64, 2)
-    else TILES_CASE(bf16_t, 64, 4)
+        if (half) TILES_CASE(bf16_t, 128, 1, 4)
+        else if (twice) TILES_CASE(bf16_t, 128, 2, 2)
+        else TILES_CASE(bf16_t, 128, 2, 4)
+    } else if (half) TILES_CASE(bf16_t, 64, 2, 4)
+    else TILES_CASE(bf16_t, 64, 4, 4)
 #undef TILES_CASE
     return mllm_check_launch("scaled_attention_tiles");
 }

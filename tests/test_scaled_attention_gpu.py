@@ -365,3 +365,19 @@ def test_a_context_at_the_end_of_all_numbers_stays_in_its_table():
     out = K.paged_attention(q, k_pages, v_pages, ints([0] * n), ints(list(range(n))), ints([[0, 1, 2, 3]]), 2, 2, 64, 0.125, max_q_len=n, max_len=256, q_starts=ints([0, n]),
                             context_lens=ints([2**31 - 3]))
     assert out.shape == (n, 128) and not bool(out.any())   # (the pages hold zeros)
+
+
+@pytest.mark.parametrize("size,page", [(128, 64), (80, 16)])
+@pytest.mark.parametrize("options", [{}, dict(window=70, keep_first=5, softcap=4.0), dict(chunk=48)], ids=["whole", "window", "chunk"])
+def test_blocks_in_plenty_take_twice_the_rows(size, page, options):
+    """Enough blocks (2,048) for the form whose waves share a block's rows between them; the last tile of the first portion has rows for half of
+    them only."""
+    batch = Batch("bf16", 104, 2, size, page, [0, 37], [520, 61], seed=size)
+    for plane in batch.planes:
+        plane.codes[batch.unused] = torch.nan
+    batch.planes[1].codes[int(batch.tables[0, 300 // page]), 0, 300 % page, 3] = torch.nan
+    got = batch.run(**options).double().cpu()
+    want = batch.want(**options)
+    lost = torch.isnan(want)
+    assert bool(lost.any()) and torch.equal(torch.isnan(got), lost)
+    close(torch.where(lost, 0.0, got), torch.where(lost, 0.0, want), batch)
