@@ -1,5 +1,5 @@
-// What the two kernels of attention over a cache of 8 bits share (scaled_attention_rows.hip, scaled_attention_tiles.hip): their arguments and what refuses them,
-// and how results are written.
+// Attention over a cache of 8 bits: what a row by itself takes and what a tile of a portion's rows does, for the kernels of either (scaled_attention_rows.hip,
+// scaled_attention_tiles.hip) and of both at once (scaled_attention_mixed.hip); their arguments, what refuses them, and how results are written.
 //
 // A token at position p attends to the keys max(0, p - window + 1) .. p of its request (window 0: all; with kept first keys also to those;
 // or, with chunks, to the keys of its own chunk up to p). A row without a request, or at a position before the first, sees nothing:
@@ -64,6 +64,168 @@ struct RowView {
     __device__ __forceinline__ bool sees() const { return request >= 0 && position >= 0; }
 };
 
+constexpr int MOST_RUNS = 1024;   // of a row: their factors lie in LDS when they are put together
+
+// How many runs a row's tiles are cut into.
+__device__ __forceinline__ int runs_of(int tiles, int run_tiles, int n_runs) { return min(ceil_div(tiles, run_tiles), n_runs); }
+
+// A row by itself (decoding, short portions, and whatever else comes without the shape of portions), its heads of set `set` (up to 16 that share a
+// key/value head), and a run of `run_tiles` tiles, by `waves` waves: they take the run's tiles in turn and meet in `meeting`
+// ([wave][column][head_size + 4]). Rows of more than one run leave unnormalised sums, maximum and weight per run in `parts` ([row, head, run,
+// head_size + 2]).
+template <typename T, int HD, bool WHOLE>
+__device__ __forceinline__ void attend_row(const AttendArguments& a, int row, int set, int run, int waves, int run_tiles, int n_runs, float* __restrict__ parts, float* meeting) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    typedef ScaledSweep<HD, 1, WIDE, false, WHOLE> Sweep;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), threads = waves * WAVE;
+    const int head_size = a.planes.head_size, group = a.n_heads / a.planes.n_kv_heads, sets = ceil_div(group, 16);
+    const int kv_head = set / sets, head0 = kv_head * group + (set % sets) * 16;
+    const int columns = min(16, (kv_head + 1) * group - head0);
+    const RowView view(a, row);
+    if (!view.sees()) {
+        if (run == 0)
+            for (int i = threadIdx.x; i < columns * head_size; i += threads) put_result<T>(a, row, head0 * head_size + i, 0.0f);
+        return;
+    }
+    const TileRange range(view.first, view.position, a.keep);
+    const int runs = runs_of(range.count, run_tiles, n_runs);
+    if (run >= runs) return;
+    const bool alone = runs == 1;
+    const int share = ceil_div(range.count, runs), begin = run * share, end = min(range.count, begin + share);   // (the runs of a row are alike)
+
+    Sweep sweep;
+    sweep.init(head_size, lane);
+    const int column = lane % 16;
+    sweep.template load_query<T>(0, column < columns ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride + (head0 + column) * head_size : nullptr, head_size, a.aligned, a.negative, lane);
+    const Columns heads = {view.position, view.position, a.window, a.chunk, a.keep};
+    sweep.tiles(range, begin + wave, waves, end, a.block_tables + (size_t)view.request * a.max_blocks, a.planes, kv_head, a.scale, heads, view.first, view.position, lane);
+
+    const int pitch = head_size + 4;
+    const float l = sweep.weight_sum(0);
+    // the maximum is the same in the four lanes of a column: it is only raised together
+    float* const mine = meeting + (wave * columns + column) * pitch;
+    if (column < columns) {
+#pragma unroll
+        for (int dt = 0; dt < Sweep::DT; dt++)
+            if (dt * 16 < head_size) *reinterpret_cast<f32x4*>(mine + dt * 16 + 4 * (lane / 16)) = sweep.o[0][dt];
+        if (lane < 16) {
+            mine[head_size] = sweep.m[0];
+            mine[head_size + 1] = l;
+        }
+    }
+    __syncthreads();
+    // a wave without tiles has m = NO_SCORE, l = 0 and sums of 0
+    for (int i = threadIdx.x; i < columns * head_size; i += threads) {
+        const int c = i / head_size, d = i % head_size;
+        const float* const at = meeting + c * pitch;
+        float top = NO_SCORE;
+        for (int w = 0; w < waves; w++) top = fmaxf(top, at[w * columns * pitch + head_size]);
+        float total = 0.0f, value = 0.0f;
+        for (int w = 0; w < waves; w++) {
+            const float factor = weight_of<WIDE>(at[w * columns * pitch + head_size] - top);
+            total += at[w * columns * pitch + head_size + 1] * factor;
+            value += at[w * columns * pitch + d] * factor;
+        }
+        if (alone) {
+            if (a.sinks) total += weight_of<WIDE>(a.sinks[head0 + c] * a.sink_factor - top);
+            put_result<T>(a, row, (head0 + c) * head_size + d, value / total);
+        } else {
+            float* const part = parts + (((size_t)row * a.n_heads + head0 + c) * n_runs + run) * (head_size + 2);
+            part[d] = value;
+            if (d == 0) {
+                part[head_size] = top;
+                part[head_size + 1] = total;
+            }
+        }
+    }
+}
+
+constexpr int MOST_ROWS = 65535 * 16;                   // of a portion in one launch
+constexpr int MOST_REACH = 2147483647 - 2 * MOST_ROWS;   // positions, the rows of a block that a portion does not have among them, are numbers of 32 bits
+
+// What the four waves of a block of a portion share: the queries' operands while keys are walked; then what the waves hold, row by row.
+template <typename T, int HD, int CT, int SPLITS>
+union TileMemory {
+    bf16x8 queries[4 / SPLITS][ScaledSweep<HD, CT, sizeof(T) == 4, true, true>::Q_PIECES];
+    float meeting[4][16 * CT][HD + 4];
+};
+
+// Rows of a portion: request, head and tile of 16 CT 4 / SPLITS rows. SPLITS of four waves take the tiles of keys in turn, each with statistics of
+// its own, and meet in LDS; with two, the other two do the same for 16 CT rows more, at the same time, so that half of what they read comes from
+// the compute unit's own cache.
+template <typename T, int HD, int CT, int SPLITS, bool WHOLE>
+__device__ __forceinline__ void attend_tile(const AttendArguments& a, int request, int head, int tile, TileMemory<T, HD, CT, SPLITS>& lds) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    typedef ScaledSweep<HD, CT, WIDE, true, WHOLE> Sweep;
+    constexpr int WAVES = 4, GROUPS = WAVES / SPLITS, WAVE_ROWS = 16 * CT, ROWS = GROUPS * WAVE_ROWS;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = wave % GROUPS, split = wave / GROUPS;
+    const int head_size = a.planes.head_size;
+    const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
+    const int row0 = tile * ROWS;
+    const int reach = (int)min((long long)a.max_blocks << a.planes.page_shift, (long long)MOST_REACH) - 1;
+    const int context = min(a.context_lens[request], reach);
+    if (row0 >= q_len || context < 0 || q_first < 0) return;   // (a negative context: a padding request, whose rows are nobody's)
+    const int kv_head = head / (a.n_heads / a.planes.n_kv_heads);
+    const int own0 = row0 + group * WAVE_ROWS;   // the wave's first row, if the portion has it
+    const int position0 = min(context + own0, reach), position1 = min(context + min(own0 + WAVE_ROWS, q_len) - 1, reach);
+
+    Sweep sweep;
+    sweep.init(head_size, lane);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const int local = own0 + 16 * ct + lane % 16;
+        const bool valid = local < q_len;
+        if (ct % SPLITS == split) {
+            sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
+            sweep.share_query(ct, lds.queries[group], lane);
+        }
+    }
+    sweep.q_shared = lds.queries[group];
+    __syncthreads();
+    if (GROUPS == 1 || own0 < q_len) {
+        const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
+        sweep.tiles(range, split, SPLITS, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale,
+                    {context + own0 + lane % 16, position1, a.window, a.chunk, a.keep}, scaled_first_key(position1, a.window, a.chunk), position0, lane);
+    }
+
+    __syncthreads();   // (all waves are through with the queries)
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        float* const mine = lds.meeting[wave][16 * ct + lane % 16];
+#pragma unroll
+        for (int dt = 0; dt < Sweep::DT; dt++) *reinterpret_cast<f32x4*>(mine + 16 * dt + 4 * (lane / 16)) = sweep.o[ct][dt];
+        const float sum = sweep.weight_sum(ct);
+        if (lane < 16) {
+            mine[HD] = sweep.m[ct];
+            mine[HD + 1] = sum;
+        }
+    }
+    __syncthreads();
+    // four elements of a row a thread, as they lie in the results
+    const int fours = head_size / 4;
+    for (int i = threadIdx.x; i < ROWS * fours; i += 256) {
+        const int row = i / fours, d = 4 * (i % fours);
+        if (row0 + row >= q_len) break;
+        const int of_group = GROUPS == 1 ? 0 : row / WAVE_ROWS, at = GROUPS == 1 ? row : row % WAVE_ROWS;
+        float top = NO_SCORE;
+#pragma unroll
+        for (int w = 0; w < SPLITS; w++) top = fmaxf(top, lds.meeting[w * GROUPS + of_group][at][HD]);
+        float total = a.sinks ? weight_of<WIDE>(a.sinks[head] * a.sink_factor - top) : 0.0f;
+        f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < SPLITS; w++) {
+            const float* const part = lds.meeting[w * GROUPS + of_group][at];
+            const float factor = weight_of<WIDE>(part[HD] - top);
+            total += part[HD + 1] * factor;
+            const f32x4 theirs = *reinterpret_cast<const f32x4*>(part + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) value[e] += theirs[e] * factor;
+        }
+        const float inverse = 1.0f / total;
+        put_four<T>(a, q_first + row0 + row, head * head_size + d, value * inverse);
+    }
+}
+
 inline int refuse_attend(const char* what, const AttendArguments& a, int page_size, int dtype) {
     const ScaledPlanes& p = a.planes;
     MLLM_REQUIRE(a.n_rows >= 0 && a.n_heads > 0 && p.n_kv_heads > 0 && a.max_blocks > 0 && a.n_tables > 0 && p.num_pages > 0, "%s: bad sizes", what);
@@ -97,3 +259,6 @@ inline AttendArguments attend_arguments(const void* q, long long q_stride, const
     a.sink_factor = unit;
     return a;
 }
+
+// Puts the runs of rows together (scaled_attention_rows.hip).
+int scaled_merge(const AttendArguments& a, int dtype, int n_rows, int run_tiles, int n_runs, const float* parts, hipStream_t stream);

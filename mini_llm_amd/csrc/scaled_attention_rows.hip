@@ -3,85 +3,14 @@
 
 namespace {
 
-constexpr int MOST_RUNS = 1024;   // of a row: their factors lie in LDS when they are put together
-
 // The most waves a block of rows may have: as many as have the registers they need.
 constexpr int rows_waves(int padded, int size) { return padded == 64 ? (size == 2 ? 16 : 8) : 1024 / padded; }
 
-// How many runs a row's tiles are cut into.
-__device__ __forceinline__ int runs_of(int tiles, int run_tiles, int n_runs) { return min(ceil_div(tiles, run_tiles), n_runs); }
-
-// Rows by themselves (decoding, short portions, and whatever else comes without the shape of portions): a block per row, group of up to 16
-// heads that share a key/value head, and run of `run_tiles` tiles; its waves take the run's tiles in turn and meet in LDS. Rows of more
-// than one run leave unnormalised sums, maximum and weight per run in `parts` ([row, head, run, head_size + 2]) for the kernel below.
-// What bounds it is the cache's bytes: 2 (head_size + 0.25) a key for all heads of the group together.
+// A block per row, set of heads and run of keys. What bounds it is the cache's bytes: 2 (head_size + 0.25) a key for all heads of a set together.
 template <typename T, int HD, bool WHOLE>
 __global__ __launch_bounds__(WAVE * rows_waves(HD, sizeof(T))) void scaled_rows_attention_kernel(AttendArguments a, int run_tiles, int n_runs, float* __restrict__ parts) {
-    constexpr bool WIDE = sizeof(T) == 4;
-    typedef ScaledSweep<HD, 1, WIDE, false, WHOLE> Sweep;
-    extern __shared__ float meeting[];   // [wave][column][head_size + 4]
-    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
-    const int row = blockIdx.x, run = blockIdx.z;
-    const int head_size = a.planes.head_size, group = a.n_heads / a.planes.n_kv_heads, sets = ceil_div(group, 16);
-    const int kv_head = blockIdx.y / sets, head0 = kv_head * group + (blockIdx.y % sets) * 16;
-    const int columns = min(16, (kv_head + 1) * group - head0);
-    const RowView view(a, row);
-    if (!view.sees()) {
-        if (run == 0)
-            for (int i = threadIdx.x; i < columns * head_size; i += blockDim.x) put_result<T>(a, row, head0 * head_size + i, 0.0f);
-        return;
-    }
-    const TileRange range(view.first, view.position, a.keep);
-    const int runs = runs_of(range.count, run_tiles, n_runs);
-    if (run >= runs) return;
-    const bool alone = runs == 1;
-    const int share = ceil_div(range.count, runs), begin = run * share, end = min(range.count, begin + share);   // (the runs of a row are alike)
-
-    Sweep sweep;
-    sweep.init(head_size, lane);
-    const int column = lane % 16;
-    sweep.template load_query<T>(0, column < columns ? static_cast<const T*>(a.q) + (size_t)row * a.q_stride + (head0 + column) * head_size : nullptr, head_size, a.aligned, a.negative, lane);
-    const Columns heads = {view.position, view.position, a.window, a.chunk, a.keep};
-    sweep.tiles(range, begin + wave, waves, end, a.block_tables + (size_t)view.request * a.max_blocks, a.planes, kv_head, a.scale, heads, view.first, view.position, lane);
-
-    const int pitch = head_size + 4;
-    const float l = sweep.weight_sum(0);
-    // the maximum is the same in the four lanes of a column: it is only raised together
-    float* const mine = meeting + (wave * columns + column) * pitch;
-    if (column < columns) {
-#pragma unroll
-        for (int dt = 0; dt < Sweep::DT; dt++)
-            if (dt * 16 < head_size) *reinterpret_cast<f32x4*>(mine + dt * 16 + 4 * (lane / 16)) = sweep.o[0][dt];
-        if (lane < 16) {
-            mine[head_size] = sweep.m[0];
-            mine[head_size + 1] = l;
-        }
-    }
-    __syncthreads();
-    // a wave without tiles has m = NO_SCORE, l = 0 and sums of 0
-    for (int i = threadIdx.x; i < columns * head_size; i += blockDim.x) {
-        const int c = i / head_size, d = i % head_size;
-        const float* const at = meeting + c * pitch;
-        float top = NO_SCORE;
-        for (int w = 0; w < waves; w++) top = fmaxf(top, at[w * columns * pitch + head_size]);
-        float total = 0.0f, value = 0.0f;
-        for (int w = 0; w < waves; w++) {
-            const float factor = weight_of<WIDE>(at[w * columns * pitch + head_size] - top);
-            total += at[w * columns * pitch + head_size + 1] * factor;
-            value += at[w * columns * pitch + d] * factor;
-        }
-        if (alone) {
-            if (a.sinks) total += weight_of<WIDE>(a.sinks[head0 + c] * a.sink_factor - top);
-            put_result<T>(a, row, (head0 + c) * head_size + d, value / total);
-        } else {
-            float* const part = parts + (((size_t)row * a.n_heads + head0 + c) * n_runs + run) * (head_size + 2);
-            part[d] = value;
-            if (d == 0) {
-                part[head_size] = top;
-                part[head_size + 1] = total;
-            }
-        }
-    }
+    extern __shared__ float meeting[];
+    attend_row<T, HD, WHOLE>(a, blockIdx.x, blockIdx.y, blockIdx.z, blockDim.x / WAVE, run_tiles, n_runs, parts, meeting);
 }
 
 // Puts the runs of a row's head together: a wave a (row, head), four to a block; eight runs' sums are on their way at a time.
@@ -128,6 +57,15 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(AttendArguments a, in
 
 }  // namespace
 
+int scaled_merge(const AttendArguments& a, int dtype, int n_rows, int run_tiles, int n_runs, const float* parts, hipStream_t stream) {
+    mllm_count_kernel(MLLM_K_SCALED_ATTENTION_MERGE);
+    const dim3 grid(n_rows, ceil_div(a.n_heads, 4));
+    const size_t lds = (size_t)4 * n_runs * sizeof(float);
+    if (dtype == MLLM_F32) scaled_merge_kernel<float><<<grid, 4 * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);
+    else scaled_merge_kernel<bf16_t><<<grid, 4 * WAVE, lds, stream>>>(a, run_tiles, n_runs, parts);
+    return mllm_check_launch("scaled_attention_merge");
+}
+
 // Rows by themselves. The keys of a row are cut into as many runs as have at most run_tiles tiles of 64 each, n_runs at most (a longer
 // sequence has longer runs, so no key is left out); n_runs > 1 needs `parts`, n_rows * n_heads * n_runs * (head_size + 2) floats.
 MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const void* k_codes, const float* k_scales, const void* v_codes, const float* v_scales, void* out,
@@ -164,11 +102,5 @@ MLLM_API int mllm_scaled_attention_rows(const void* q, long long q_stride, const
 #undef ROWS_CASE
 #undef ROWS_LAUNCH
     if (int status = mllm_check_launch("scaled_attention_rows")) return status;
-    if (n_runs == 1) return 0;
-    mllm_count_kernel(MLLM_K_SCALED_ATTENTION_MERGE);
-    const dim3 merge_grid(n_rows, ceil_div(n_heads, 4));
-    const size_t merge_lds = (size_t)4 * n_runs * sizeof(float);
-    if (dtype == MLLM_F32) scaled_merge_kernel<float><<<merge_grid, 4 * WAVE, merge_lds, stream>>>(a, run_tiles, n_runs, parts);
-    else scaled_merge_kernel<bf16_t><<<merge_grid, 4 * WAVE, merge_lds, stream>>>(a, run_tiles, n_runs, parts);
-    return mllm_check_launch("scaled_attention_merge");
+    return n_runs == 1 ? 0 : scaled_merge(a, dtype, n_rows, run_tiles, n_runs, parts, stream);
 }

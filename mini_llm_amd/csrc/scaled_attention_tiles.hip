@@ -5,89 +5,11 @@
 
 namespace {
 
-constexpr int MOST_ROWS = 65535 * 16;                   // of a portion in one launch
-constexpr int MOST_REACH = 2147483647 - 2 * MOST_ROWS;   // positions, the rows of a block that a portion does not have among them, are numbers of 32 bits
-
-// Portions of prompts: a block per (request, head, tile of rows). SPLITS of its four waves take the tiles of keys in turn, each with statistics of
-// its own, and meet in LDS; with two, the other two do the same for 16 CT rows more, at the same time, so that half of what they read comes from
-// the compute unit's own cache. Tiles with the most keys of all heads come first.
+// A block per (request, head, tile of rows). Tiles with the most keys of all heads come first.
 template <typename T, int HD, int CT, int SPLITS, bool WHOLE>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention_kernel(AttendArguments a) {
-    constexpr bool WIDE = sizeof(T) == 4;
-    typedef ScaledSweep<HD, CT, WIDE, true, WHOLE> Sweep;
-    constexpr int WAVES = 4, GROUPS = WAVES / SPLITS, WAVE_ROWS = 16 * CT, ROWS = GROUPS * WAVE_ROWS;
-    // the queries' operands while keys are walked; then what the waves hold, row by row
-    constexpr int PITCH = HD + 4;
-    __shared__ union {
-        bf16x8 queries[GROUPS][Sweep::Q_PIECES];
-        float meeting[WAVES][WAVE_ROWS][PITCH];
-    } lds;
-    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = wave % GROUPS, split = wave / GROUPS;
-    const int request = blockIdx.z, head = blockIdx.x, head_size = a.planes.head_size;
-    const int q_first = a.q_starts[request], q_len = min(a.q_starts[request + 1], a.n_rows) - q_first;
-    const int row0 = (gridDim.y - 1 - blockIdx.y) * ROWS;
-    const int reach = (int)min((long long)a.max_blocks << a.planes.page_shift, (long long)MOST_REACH) - 1;
-    const int context = min(a.context_lens[request], reach);
-    if (row0 >= q_len || context < 0 || q_first < 0) return;   // (a negative context: a padding request, whose rows are nobody's)
-    const int kv_head = head / (a.n_heads / a.planes.n_kv_heads);
-    const int own0 = row0 + group * WAVE_ROWS;   // the wave's first row, if the portion has it
-    const int position0 = min(context + own0, reach), position1 = min(context + min(own0 + WAVE_ROWS, q_len) - 1, reach);
-
-    Sweep sweep;
-    sweep.init(head_size, lane);
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        const int local = own0 + 16 * ct + lane % 16;
-        const bool valid = local < q_len;
-        if (ct % SPLITS == split) {
-            sweep.template load_query<T>(ct, valid ? static_cast<const T*>(a.q) + (size_t)(q_first + local) * a.q_stride + head * head_size : nullptr, head_size, a.aligned, a.negative, lane);
-            sweep.share_query(ct, lds.queries[group], lane);
-        }
-    }
-    sweep.q_shared = lds.queries[group];
-    __syncthreads();
-    if (GROUPS == 1 || own0 < q_len) {
-        const TileRange range(scaled_first_key(position0, a.window, a.chunk), position1, a.keep);
-        sweep.tiles(range, split, SPLITS, range.count, a.block_tables + (size_t)request * a.max_blocks, a.planes, kv_head, a.scale,
-                    {context + own0 + lane % 16, position1, a.window, a.chunk, a.keep}, scaled_first_key(position1, a.window, a.chunk), position0, lane);
-    }
-
-    __syncthreads();   // (all waves are through with the queries)
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        float* const mine = lds.meeting[wave][16 * ct + lane % 16];
-#pragma unroll
-        for (int dt = 0; dt < Sweep::DT; dt++) *reinterpret_cast<f32x4*>(mine + 16 * dt + 4 * (lane / 16)) = sweep.o[ct][dt];
-        const float sum = sweep.weight_sum(ct);
-        if (lane < 16) {
-            mine[HD] = sweep.m[ct];
-            mine[HD + 1] = sum;
-        }
-    }
-    __syncthreads();
-    // four elements of a row a thread, as they lie in the results
-    const int fours = head_size / 4;
-    for (int i = threadIdx.x; i < ROWS * fours; i += blockDim.x) {
-        const int row = i / fours, d = 4 * (i % fours);
-        if (row0 + row >= q_len) break;
-        const int of_group = GROUPS == 1 ? 0 : row / WAVE_ROWS, at = GROUPS == 1 ? row : row % WAVE_ROWS;
-        float top = NO_SCORE;
-#pragma unroll
-        for (int w = 0; w < SPLITS; w++) top = fmaxf(top, lds.meeting[w * GROUPS + of_group][at][HD]);
-        float total = a.sinks ? weight_of<WIDE>(a.sinks[head] * a.sink_factor - top) : 0.0f;
-        f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < SPLITS; w++) {
-            const float* const part = lds.meeting[w * GROUPS + of_group][at];
-            const float factor = weight_of<WIDE>(part[HD] - top);
-            total += part[HD + 1] * factor;
-            const f32x4 theirs = *reinterpret_cast<const f32x4*>(part + d);
-#pragma unroll
-            for (int e = 0; e < 4; e++) value[e] += theirs[e] * factor;
-        }
-        const float inverse = 1.0f / total;
-        put_four<T>(a, q_first + row0 + row, head * head_size + d, value * inverse);
-    }
+    __shared__ TileMemory<T, HD, CT, SPLITS> lds;
+    attend_tile<T, HD, CT, SPLITS, WHOLE>(a, blockIdx.z, blockIdx.x, gridDim.y - 1 - blockIdx.y, lds);
 }
 
 }  // namespace

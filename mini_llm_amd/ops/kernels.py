@@ -1664,10 +1664,20 @@ def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int, wide: bool
     return waves, run, runs
 
 
+def scaled_mixes(row_blocks: int, rows: int, requests: int, longest: int, n_heads: int, head_size: int, wide: bool = False) -> bool:
+    """Whether a step's decoding rows (``row_blocks`` (row, head group) pairs) and its portions (``rows`` of ``requests``, up to ``longest`` each) go in one launch over
+    pages of 8 bits. There the portions' blocks have half the rows that they may have by themselves, and rows four waves."""
+    # us in one / two launches (and a merge where rows are cut), 12 heads of 64 in bfloat16, rows at 900 keys beside a portion of 512: 1 row 7.1 / 13.0, 8 8.3 / 15.1, 32 15.5 / 18.9,
+    # 64 23.0 / 26.5, 128 (1,536 pairs) 43.4 / 46.3, 256 77.7 / 77.1; 32 rows beside 2,048 (384 blocks of whole tiles) 26.6 / 31.3; 32 heads of 128 on 8, 16 rows at 2,000 beside 512 (512
+    # blocks) 31.9 / 31.1, 32 beside 2,048 (2,048) 113 / 86; in 32-bit 12 heads of 64, 64 rows beside 512 24.4 / 29.4.
+    tile = 64 if head_size <= 64 and not wide else 32
+    return head_size <= 128 and row_blocks <= 2048 and n_heads * min(rows // tile + requests, requests * -(-longest // tile)) <= 512
+
+
 def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_tables, n_heads, n_kv_heads, head_size, scale, window, max_q_len, max_len, q_starts, context_lens, out,
                       short_rows, short_requests, packed_out, softcap, sinks, chunk, keep_first, wide_out):
     """``paged_attention`` over pages of 8 bits: rows by themselves (decoding, short portions, batches without the shape of portions) a block per
-    row and group of heads; portions a block per head and tile of rows."""
+    row and group of heads; portions a block per head and tile of rows; a step of both in one launch where that pays."""
     here = _check_scaled(k_pages, v_pages, n_kv_heads, head_size)
     num_pages, _, page_size, _ = k_pages.shape
     _require(n_heads > 0 and n_heads % n_kv_heads == 0, f"{n_heads} heads do not divide into {n_kv_heads} key/value heads")
@@ -1698,14 +1708,18 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
     table_at = block_tables.data_ptr()
     given = (q.data_ptr(), stride, *k_pages.addresses, *v_pages.addresses)
 
-    def rows_alone(count, into, packed):
+    def cut_of(count):
+        """scaled_cut for so many rows, and memory for what their runs leave."""
         reach = max_blocks * page_size
         span = min(window + keep if window else chunk or reach, reach)
         tiles = -(-span // SCALED_TILE) + (2 if window or chunk else 0)
         if max_len is not None:   # (what lies beyond it is the last run's)
             tiles = max(1, min(tiles, -(-int(max_len) // SCALED_TILE)))
         waves, run, runs = scaled_cut(count * n_kv_heads * -(-group // 16), tiles, head_size, min(16, group), code == F32)
-        parts = torch.empty((count, n_heads, runs, head_size + 2), dtype=torch.float32, device=q.device) if runs > 1 else None
+        return waves, run, runs, torch.empty((count, n_heads, runs, head_size + 2), dtype=torch.float32, device=q.device) if runs > 1 else None
+
+    def rows_alone(count, into, packed):
+        waves, run, runs, parts = cut_of(count)
         check(lib.mllm_scaled_attention_rows(*given, into.data_ptr(), width if packed else out_stride, request_at, position_at, table_at, max_blocks, n_tables, num_pages, count,
                                              n_heads, n_kv_heads, head_size, page_size, window, scale, code, softcap, sink_at, chunk, keep, wide_out, packed, waves, run, runs,
                                              _ptr(parts), _stream()))
@@ -1724,6 +1738,12 @@ def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_table
     skipped = 0
     if short_rows is not None and short_requests is not None and 0 < short_rows < n:
         _require(0 < short_requests < n_requests, "short_requests does not cut the batch in two")
+        if scaled_mixes(int(short_rows) * n_kv_heads * -(-group // 16), n - int(short_rows), n_requests - int(short_requests), int(max_q_len), n_heads, head_size, code == F32):
+            _, run, runs, parts = cut_of(int(short_rows))
+            check(lib.mllm_scaled_attention_mixed(*given, out.data_ptr(), out_stride, request_at, position_at, start_at, context_at, table_at, max_blocks, n_tables, num_pages, n, n_heads,
+                                                  n_kv_heads, head_size, page_size, window, scale, code, softcap, sink_at, chunk, keep, wide_out, int(short_rows), int(short_requests),
+                                                  n_requests, int(max_q_len), run, runs, _ptr(parts), _stream()))
+            return out
         rows_alone(int(short_rows), out, False)
         skipped = int(short_requests)
     check(lib.mllm_scaled_attention_tiles(*given, out.data_ptr(), out_stride, start_at + 4 * skipped, context_at + 4 * skipped, table_at + 4 * skipped * max_blocks, max_blocks,

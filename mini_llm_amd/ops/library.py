@@ -118,6 +118,7 @@ _SIGNATURES = {
                                    c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],
     "mllm_scaled_attention_tiles": [P, c_longlong, P, P, P, P, P, c_longlong, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_float,
                                     P, c_int, c_int, c_int, P],
+    "mllm_scaled_attention_mixed": [P, c_longlong, P, P, P, P, P, c_longlong, P, P, P, P, P, *[c_int] * 9, c_float, c_int, c_float, P, *[c_int] * 9, P, P],
     "mllm_recurrence_chunk_rows": [c_int],
     "mllm_recurrence_chunked": [c_int, P, c_int, P, c_int, P, c_int, P, P, c_int, c_float, P, c_float, P, c_longlong, c_longlong, c_longlong, P, P, P, c_int,
                                 c_int, c_int, c_int, c_int, c_int, P, c_longlong, c_int, P],

@@ -381,3 +381,29 @@ def test_blocks_in_plenty_take_twice_the_rows(size, page, options):
     lost = torch.isnan(want)
     assert bool(lost.any()) and torch.equal(torch.isnan(got), lost)
     close(torch.where(lost, 0.0, got), torch.where(lost, 0.0, want), batch)
+
+
+@pytest.mark.parametrize("one", [True, False], ids=["one-launch", "two-launches"])
+@pytest.mark.parametrize("dtype,heads,kv_heads,size,page", [("bf16", 4, 2, 64, 64), ("bf16", 20, 1, 48, 16), ("bf16", 3, 3, 128, 32), ("bf16", 4, 1, 80, 128), ("f32", 4, 2, 64, 16),
+                                                            ("f32", 18, 1, 128, 64)])
+@pytest.mark.parametrize("options", [{}, dict(window=70, keep_first=5, softcap=4.0), dict(chunk=48)], ids=["whole", "window", "chunk"])
+def test_a_step_of_rows_and_portions(dtype, heads, kv_heads, size, page, options, one, monkeypatch):
+    """Rows that are cut into runs and put together (the first is long) beside portions, in one launch and in two."""
+    monkeypatch.setattr(kernels(), "scaled_mixes", lambda *a: one)
+    batch = Batch(dtype, heads, kv_heads, size, page, [2600, 7, 0, 60, 0], [1, 3, 1, 40, 100], seed=size)
+    before = kernels().launch_counts()
+    got = batch.run(short_rows=5, short_requests=3, **options)
+    ran = kernels().launches_since(before)
+    assert ("scaled_attention_mixed" in ran) == one and ("scaled_attention_tiles" in ran) != one
+    check(batch, got, **options)
+
+
+def test_a_step_of_both_kinds_with_numbers_that_are_none():
+    batch = Batch("bf16", 4, 2, 64, 64, [130, 7, 60, 0], [1, 1, 40, 100], seed=3)
+    for plane in batch.planes:
+        plane.codes[batch.unused] = torch.nan
+    batch.planes[1].codes[int(batch.tables[2, 1]), 0, 10, 3] = torch.nan   # position 74 of the third request: seen by the later rows of its portion
+    got, want = batch.run(short_rows=2, short_requests=2).double().cpu(), batch.want()
+    lost = torch.isnan(want)
+    assert bool(lost.any()) and torch.equal(torch.isnan(got), lost)
+    close(torch.where(lost, 0.0, got), torch.where(lost, 0.0, want), batch)
