@@ -3,7 +3,8 @@
 
 namespace {
 
-// The blocks of rows first, then those of tiles of rows, each as in its own kernel: either part's wait for its longest block runs under the other's blocks.
+// The blocks of rows first, then those of tiles of rows, each as in its own kernel: either part's wait for its longest block runs under the other's blocks
+// (33 rows beside three portions, float32, 12 heads of 64: 24.5 us in two launches, 16.4 in one).
 template <typename T, int HD, int CT, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void scaled_mixed_attention_kernel(AttendArguments a, int short_rows, int sets, int n_runs, int run_tiles, float* __restrict__ parts,
                                                                         int short_requests, int n_tiles) {

@@ -5,7 +5,10 @@
 
 namespace {
 
-// A block per (request, head, tile of rows). Tiles with the most keys of all heads come first.
+// A block per (request, head, tile of rows). Tiles with the most keys of all heads come first. What bounds it: a wave issues its own conversions, softmax
+// arithmetic and products one behind the other, and two waves a SIMD (what 250 registers leave) overlap in part: 16 heads of 128 on 8,192 rows 286 us, 961 TFLOP/s
+// of the keys that are seen (vector instructions in half the cycles, matrix instructions in a third); without the exponentials it would be 5 % less, without the reads of keys and values 22 %. 12 heads of 64 on 2,048
+// rows 20 us, where the launch is one round of blocks and the longest has eight tiles of keys a wave.
 template <typename T, int HD, int CT, int SPLITS, bool WHOLE>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention_kernel(AttendArguments a) {
     __shared__ TileMemory<T, HD, CT, SPLITS> lds;
