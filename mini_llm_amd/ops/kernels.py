@@ -1659,7 +1659,7 @@ def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int, wide: bool
     runs = -(-tiles // run)
     # Waves: as many as have a tile, up to 12 a compute unit (768 blocks of 16 tiles with 2 / 4 / 8 waves 15.5 / 15.3 / 17.3; 512 14.3 / 12.4 / 13.0).
     waves = 1
-    while waves < most and waves < run and 2 * waves * blocks * runs <= 3072:
+    while waves < most and waves < run and 2 * waves * blocks * runs <= 12 * 256:
         waves *= 2
     return waves, run, runs
 
