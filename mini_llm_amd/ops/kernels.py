@@ -499,7 +499,7 @@ def paged_attention(q, k_pages, v_pages, token_request, positions, block_tables,
     products are as exact as that type's (what is held in 8 bits is exact in bfloat16).
     ``first_row``: where the rows are a part of a step's batch whose other parts may run at the same time on other
     streams, the place of the first of them in the whole batch (kernels that keep counters per row keep them apart by it)."""
-    if isinstance(k_pages, ScaledPages):
+    if isinstance(k_pages, ScaledPages) or isinstance(v_pages, ScaledPages):
         return _scaled_attention(q, k_pages, v_pages, token_request, positions, block_tables, n_heads, n_kv_heads, head_size, float(scale), int(window or 0), max_q_len, max_len,
                                  q_starts, context_lens, out, short_rows, short_requests, packed_out, float(softcap or 0.0), sinks, int(chunk or 0), int(keep_first or 0), bool(wide_out))
     _check_pages(k_pages, v_pages, n_kv_heads, head_size)

@@ -103,3 +103,18 @@ def test_bookkeeping_of_a_cache_of_8_bits():
 
     cache = CacheManager([CacheGroupSpec("g", (0, 1), 2, 32, None)], {}, num_pages=4, page_size=16, max_requests=2, device="cpu", max_length=64, scaled=True)
     assert cache.k_pages[0].is_keys and not cache.v_pages[1].is_keys and cache.k_pages[1].shape == (4, 2, 16, 32)
+
+
+def test_plain_key_pages_beside_value_pages_of_8_bits_are_refused():
+    _, v = K.scaled_pages(1, 1, 16, 16, "cpu")
+    ints = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(K.OperandError, match="8 bits"):
+        K.paged_attention(torch.zeros((1, 16)), torch.zeros((1, 1, 16, 16)), v, ints, ints, ints[None], 1, 1, 16, 0.25)
+
+
+@pytest.mark.parametrize("rows,requests,longest,heads,size,wide,one", [
+    (64, 1, 64, 12, 64, False, True), (2048, 1, 2048, 12, 64, False, True), (8192, 1, 8192, 12, 64, False, False),
+    (2048, 1, 2048, 32, 128, False, False), (512, 4, 128, 8, 256, False, False), (64, 1, 64, 12, 64, True, True)])
+def test_steps_of_both_kinds_go_in_one_launch_where_the_portions_are_few(rows, requests, longest, heads, size, wide, one):
+    assert K.scaled_mixes(12, rows, requests, longest, heads, size, wide) == one
+    assert not K.scaled_mixes(100000, rows, requests, longest, heads, size, wide)
