@@ -71,14 +71,15 @@ __device__ __forceinline__ bf16x8 eight_numbers(uint32_t lo, uint32_t hi, float 
 __device__ __forceinline__ uint32_t not_numbers(uint32_t codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // Rows of a call that fall into one block: they are neighbours and their slots follow each other. Lane i of a wave looks at row `from` + i (32 of them are
-// enough: a run has at most 16 rows); the bits of the result are the rows that begin a run, rows behind the last among them. A row
-// that goes nowhere (its slot is negative, or lies behind the pages) is a run of its own.
+// enough: a run has at most 16 rows); the bits of the result are the rows that begin a run, rows behind the last among them. Rows
+// that go nowhere (their slots are negative, or lie behind the pages) are runs of their own, as many neighbours as up to the next multiple of 16.
 __device__ __forceinline__ uint32_t run_begins(const int* __restrict__ slots, int from, int n_rows, long long n_slots, int lane) {
     const int row = from + (lane & 31);
     bool begins = true;
     if (row < n_rows && row > 0) {
         const int slot = slots[row], before = slots[row - 1];
-        begins = slot < 0 || before < 0 || slot >= n_slots || before >= n_slots || slot / BLOCK_TOKENS != before / BLOCK_TOKENS || slot != before + 1;
+        const bool nowhere = slot < 0 || slot >= n_slots, before_nowhere = before < 0 || before >= n_slots;
+        begins = nowhere != before_nowhere || (nowhere ? row % BLOCK_TOKENS == 0 : slot / BLOCK_TOKENS != before / BLOCK_TOKENS || slot != before + 1);
     }
     return (uint32_t)__ballot(begins);
 }

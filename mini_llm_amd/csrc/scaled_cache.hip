@@ -434,7 +434,7 @@ __device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const
     if (lane == 0) a.k_scales[block] = two_to(scale.exponent);
 }
 
-// A block of threads: a run of rows after another (those that begin in its `per` rows). The cosines and sines of the run's positions are made
+// A block of threads: a run of rows after another (those that begin in its rows: one each of the first `singles`, then `most`). The cosines and sines of the run's positions are made
 // once for all heads; then every wave takes heads: keys, values, queries.
 // A head of a run is one wave's, because a block has one scale: the largest magnitude is a reduction inside the wave, and what is held in front of the
 // new tokens is rounded again by who knows the new scale. Few rows: bound by the chain of dependent steps (slots, positions, cosines in 64-bit, rows, the block's scale, codes) behind
@@ -442,10 +442,11 @@ __device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const
 // and written at 3.4 TB/s (a large copy: 4.7); vector instructions are issued in half the cycles, the 64-bit turns of keys among them, and at three waves a SIMD the rest is not hidden behind
 // them. Asking for a wave's next head while it works on one takes the registers of the occupancy: 82 us for 72 with the read-back.
 template <typename T, int E, bool PIECES>
-__global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_append_kernel(AppendArguments a, int per) {
+__global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_append_kernel(AppendArguments a, int singles, int most) {
     extern __shared__ double2 tables[];   // of queries and keys, of values, and of queries in 32 bits
     const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), waves = blockDim.x / WAVE;
-    const int window = blockIdx.x * per;
+    const bool single = (int)blockIdx.x < singles;
+    const int per = single ? 1 : most, window = single ? blockIdx.x : singles + ((int)blockIdx.x - singles) * most;
     const bool keeps = a.k_at >= 0;
     // (queries alone have no blocks: any rows are a run)
     uint32_t begins = keeps ? run_begins(a.slots, window, a.n_rows, a.n_slots, lane) : per == 1 ? 0xffffffffu : 0x00010001u;
@@ -522,8 +523,9 @@ __global__ __launch_bounds__(256) void scaled_rows_kernel(const uint8_t* __restr
         const int slot = slots[first];
         T* const k_to = k_out + (size_t)first * row_size + head * head_size;
         T* const v_to = v_out + (size_t)first * row_size + head * head_size;
-        if (slot < 0 || slot >= n_slots) {   // a run of one row
-            for (int d = lane; d < head_size; d += WAVE) k_to[d] = v_to[d] = from_float<T>(0.0f);
+        if (slot < 0 || slot >= n_slots) {
+            for (int t = 0; t < count; t++)
+                for (int d = lane; d < head_size; d += WAVE) k_to[t * row_size + d] = v_to[t * row_size + d] = from_float<T>(0.0f);
             continue;
         }
         const int lead = slot % BLOCK_TOKENS;
@@ -578,7 +580,7 @@ int shift_of(int page_size) {
 MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, int k_at, int v_at, const float* q_gain, const float* k_gain, float eps, int unit,
                                 const double* frequencies, int rot_dims, int neighbours, const double* v_frequencies, int v_rot_dims, int v_neighbours,
                                 const int* positions, const int* slots, void* q_out, void* k_codes, float* k_scales, void* v_codes, float* v_scales, int num_pages,
-                                int n_rows, int n_heads, int n_kv_heads, int dim, int vdim, int head_size, int page_size, int dtype, int q_dtype,
+                                int n_rows, int n_heads, int n_kv_heads, int dim, int vdim, int head_size, int page_size, int dtype, int q_dtype, int short_rows,
                                 hipStream_t stream) {
     MLLM_REQUIRE(n_rows >= 0 && n_heads > 0 && n_kv_heads > 0 && num_pages > 0, "scaled_append: bad sizes");
     MLLM_REQUIRE(head_size > 0 && head_size % 16 == 0 && head_size <= SCALED_MAX_HEAD && dim > 0 && dim <= head_size && vdim > 0 && vdim <= head_size,
@@ -600,18 +602,21 @@ MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, in
     const int size = dtype == MLLM_F32 ? 4 : 2;
     const bool on_pieces = (uintptr_t)rows % 16 == 0 && stride * size % 16 == 0 && dim % 16 == 0 && rot_dims % 16 == 0 && (q_at < 0 || (q_at * size % 16 == 0 && (uintptr_t)q_out % 16 == 0)) &&
                            (k_at < 0 || k_at * size % 16 == 0);
-    // many rows: 16 to a block of threads, which finds the runs among them; few: a block each, so that each is under way at once. Queries alone, 32 heads of 128 turned, us with
-    // one row / 16 a block: 32 rows 5.5 / 6.4, 64 6.0 / 6.4, 128 9.4 / 6.5, 8,192 202 / 32.6.
+    // many rows: 16 to a block of threads, which finds the runs among them; few, or those that the caller says are of many requests: a block each, so that each
+    // is under way at once. 32 rows of as many requests in front of 2,016 of a prompt, keys and values of 16 heads of 64, us without / with being told: 53 / 8.8
+    // (2,048 of a prompt alone 7.0); 512 single rows 32.5 / 15.6; 32 and 480 of 32 + 16 heads of 128, turned, with queries 75 / 11.3. Queries
+    // alone, 32 heads of 128 turned, us with one row / 16 a block: 32 rows 5.5 / 6.4, 64 6.0 / 6.4, 128 9.4 / 6.5, 8,192 202 / 32.6.
     const int per = n_rows >= (k_at >= 0 ? 256 : 96) ? BLOCK_TOKENS : 1;
-    const int blocks = ceil_div(n_rows, per);
+    const int singles = per == 1 || k_at < 0 ? 0 : std::max(0, std::min(short_rows, n_rows));
+    const int blocks = singles + ceil_div(n_rows - singles, per);
     const int jobs = (k_at >= 0 ? 2 * n_kv_heads : 0) + (q_at < 0 ? 0 : on_pieces ? n_heads : n_heads * per);
     const int shares = std::max(1, std::min(ceil_div(APPEND_BLOCKS, blocks), jobs / 4));
     const dim3 grid(blocks, shares);
     const size_t lds = (size_t)BLOCK_TOKENS * (turn_pitch(rot_dims / 2) * (sizeof(double2) + sizeof(float2)) + turn_pitch(v_rot_dims / 2) * sizeof(double2));
     mllm_count_kernel(MLLM_K_SCALED_APPEND);
 #define APPEND_CASE(T, E)                                                              \
-    if (on_pieces) scaled_append_kernel<T, E, true><<<grid, 256, lds, stream>>>(a, per); \
-    else scaled_append_kernel<T, E, false><<<grid, 256, lds, stream>>>(a, per);
+    if (on_pieces) scaled_append_kernel<T, E, true><<<grid, 256, lds, stream>>>(a, singles, per); \
+    else scaled_append_kernel<T, E, false><<<grid, 256, lds, stream>>>(a, singles, per);
     if (dtype == MLLM_F32) {
         if (head_size <= 64) { APPEND_CASE(float, 1) }
         else if (head_size <= 128) { APPEND_CASE(float, 2) }

@@ -1583,7 +1583,7 @@ def _rotation(frequencies, dims: int, most: int, pairing: str, name: str, here: 
 
 def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_pages, v_pages, slots, positions, n_heads: int, n_kv_heads: int, dim: int, vdim: int, *, q_gain=None,
                   k_gain=None, unit: bool = False, eps: float = 0.0, frequencies=None, rot_dims: int = 0, pairing: str = "half", v_frequencies=None, v_rot_dims: int = 0,
-                  v_pairing: str = "half", out_dtype=None):
+                  v_pairing: str = "half", out_dtype=None, short_rows: int = 0):
     """The row-wise work between a mixer's input product and its attention over pages of 8 bits (``ScaledPages``), in one kernel. ``rows``
     (float32 or bfloat16; rows may be strided): the queries [n_heads, dim] at column ``q_at`` (None: no queries are made), the keys [n_kv_heads, dim]
     at ``k_at`` and the values [n_kv_heads, vdim] at ``v_at`` (both None: the layer reads pages another layer keeps, and only its queries are
@@ -1594,7 +1594,8 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     Keys and values of row r go to slots[r] = page * page_size + offset (negative, or behind the pages: nowhere). Rows whose slots fall into
     one block are neighbours and follow each other, as a request's tokens do, and no slot is named twice. A block whose first token
     is written begins afresh; a block that is carried on keeps its scale or, if the new rows need a larger one, is taken to that (its earlier
-    tokens' codes rounded again). Tokens of a block behind those written stay as they are.
+    tokens' codes rounded again). Tokens of a block behind those written stay as they are. ``short_rows``: the first so many rows are of many requests
+    (as ``paged_attention`` has them); it says how the work is best cut and changes no result.
 
     Returns the queries [rows, n_heads * head_size] of ``out_dtype`` (default: the rows' type), zeros behind their ``dim`` elements (None without ``q_at``)."""
     num_pages, _, page_size, head_size = k_pages.shape
@@ -1622,7 +1623,7 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     q = rows.new_empty((n, n_heads * head_size), dtype=out_dtype) if makes else None
     check(library().mllm_scaled_append(rows.data_ptr(), stride, q_at if makes else -1, k_at if keeps else -1, v_at if keeps else -1, q_gain, k_gain, eps, bool(unit), frequencies,
                                        rot_dims, pairing == "neighbours", v_frequencies, v_rot_dims, v_pairing == "neighbours", position_at, slot_at, _ptr(q), *k_pages.addresses,
-                                       *v_pages.addresses, num_pages, n, n_heads, n_kv_heads, dim, vdim, head_size, page_size, _code(rows.dtype), _code(out_dtype), _stream()))
+                                       *v_pages.addresses, num_pages, n, n_heads, n_kv_heads, dim, vdim, head_size, page_size, _code(rows.dtype), _code(out_dtype), int(short_rows), _stream()))
     return q
 
 

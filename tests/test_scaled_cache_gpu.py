@@ -257,3 +257,45 @@ def test_the_widest_heads_turned_whole(dtype, dim):
     planes[1].append(turned(wide[:, 3 * dim :].reshape(n, 2, dim), positions, f, dim, "neighbours"), slots)
     for got, plane in zip(held_by(k_pages, v_pages), planes):
         same(got, plane.held())
+
+
+@pytest.mark.parametrize("queries", [True, False])
+@pytest.mark.parametrize("told", [0, 5, 17, 20, 31, 400, 10**6], ids=str)
+def test_being_told_of_single_rows_changes_no_result(told, queries):
+    """Single rows, a portion that begins inside a block, rows that go nowhere, another portion: cut anywhere."""
+    heads, size, page = 2, 64, 32
+    starts, counts = [7, 16, 0, 31] * 5 + [5, 40], [1, 1, 1, 1] * 5 + [150, 100]
+    slots, planes = prepared(starts, counts, page, heads, size, 21)
+    slots = slots[:20] + [-1] * 37 + slots[20:170] + [2**31 - 1] * 3 + slots[170:]
+    n = len(slots)
+    g = torch.Generator().manual_seed(told % 1000)
+    rows = torch.randn((n, 4 * heads * size), generator=g) * torch.exp(torch.randn((n, 1), generator=g))
+    positions = torch.arange(n, dtype=torch.int32)
+    f = 10000.0 ** (-torch.arange(16, dtype=torch.float64) / 16)
+    k_pages, v_pages = pages_of(planes)
+    width = heads * size
+    q = kernels().scaled_append(rows.to(DEVICE), 0 if queries else None, 2 * width, 3 * width, k_pages, v_pages, torch.tensor(slots, dtype=torch.int32, device=DEVICE),
+                                positions.to(DEVICE), 2 * heads, heads, size, size, frequencies=f.to(DEVICE), rot_dims=32, short_rows=told)
+    wide = rows.double()
+    if queries:
+        want = turned(wide[:, : 2 * width].reshape(n, 2 * heads, size), positions, f, 32, "half")
+        assert bool(((q.cpu().double().view(n, 2 * heads, size) - want).abs() <= 2.0**-24 * want.abs() + 2.0**-21 * rows.abs().amax()).all())
+    planes[0].append(turned(wide[:, 2 * width : 3 * width].reshape(n, heads, size), positions, f, 32, "half"), slots)
+    planes[1].append(wide[:, 3 * width :].reshape(n, heads, size), slots)
+    for got, plane in zip(held_by(k_pages, v_pages), planes):
+        same(got, plane.held())
+
+
+@pytest.mark.parametrize("n", [3, 40, 5000])
+def test_rows_that_name_no_place_read_as_zeros(n):
+    K = kernels()
+    k_pages, v_pages = pages_of(prepared([0], [64], 32, 4, 64, 2)[1])
+    total = k_pages.shape[0] * 32
+    slots = torch.arange(n, dtype=torch.int32) % total
+    nowhere = (torch.arange(n) // 3) % 2 == 1
+    slots[nowhere] = torch.where(torch.arange(n)[nowhere] % 2 == 0, -1, total).int()
+    k, v = K.scaled_rows(k_pages, v_pages, slots.to(DEVICE))
+    everything = K.scaled_rows(k_pages, v_pages, torch.arange(total, dtype=torch.int32, device=DEVICE))
+    for got, whole in zip((k, v), everything):
+        assert not bool(got[nowhere].any())
+        assert torch.equal(got[~nowhere], whole[slots[~nowhere].long()])
