@@ -1669,10 +1669,11 @@ def scaled_mixes(row_blocks: int, rows: int, requests: int, longest: int, n_head
     """Whether a step's decoding rows (``row_blocks`` (row, head group) pairs) and its portions (``rows`` of ``requests``, up to ``longest`` each) go in one launch over
     pages of 8 bits. There the portions' blocks have half the rows that they may have by themselves, and rows four waves."""
     # us in one / two launches (and a merge where rows are cut), 12 heads of 64 in bfloat16, rows at 900 keys beside a portion of 512: 1 row 7.1 / 13.0, 8 8.3 / 15.1, 32 15.5 / 18.9,
-    # 64 23.0 / 26.5, 128 (1,536 pairs) 43.4 / 46.3, 256 77.7 / 77.1; 32 rows beside 2,048 (384 blocks of whole tiles) 26.6 / 31.3; 32 heads of 128 on 8, 16 rows at 2,000 beside 512 (512
-    # blocks) 31.9 / 31.1, 32 beside 2,048 (2,048) 113 / 86; in 32-bit 12 heads of 64, 64 rows beside 512 24.4 / 29.4.
-    tile = 64 if head_size <= 64 and not wide else 32
-    return head_size <= 128 and row_blocks <= 2048 and n_heads * min(rows // tile + requests, requests * -(-longest // tile)) <= 512
+    # 64 23.0 / 26.5, 128 (1,536 pairs) 43.4 / 46.3, 256 77.7 / 77.1; 32 rows beside 2,048 (384 blocks of whole tiles) 26.6 / 31.3, 20 heads (640) 40.1 / 45.1, 25 (800) 52.7 / 54.1, with 64 rows
+    # 71.4 / 70.6; 32 heads of 128 on 8, 16 rows at 2,000 beside 512 (512 blocks) 31.9 / 31.1, 32 beside 1,024 (1,024) 63.6 / 58.6, 2,048 (2,048) 113 / 86; in 32-bit (whose tiles are as
+    # large in either, or lose less) 64 rows beside 512 24.4 / 29.4, 25 heads, 32 rows beside 2,016 (1,600) 79.8 / 90.5, 32 heads of 128 beside 1,024 (1,024) 76.6 / 82.8.
+    tile, most = (32, 2048) if wide else (64, 832) if head_size <= 64 else (32, 512)
+    return head_size <= 128 and row_blocks <= 2048 and n_heads * min(rows // tile + requests, requests * -(-longest // tile)) <= most
 
 
 def _scaled_attention(q, k_pages, v_pages, token_request, positions, block_tables, n_heads, n_kv_heads, head_size, scale, window, max_q_len, max_len, q_starts, context_lens, out,
