@@ -207,3 +207,26 @@ def test_command_line(tmp_path, capsys):
     plain_gpt2.write_safetensors(tmp_path / "model.safetensors", plain_gpt2.random_weights(config, 3))
     assert main(["--model", str(tmp_path), "--tokens", "5,17,3", "--max-new-tokens", "6", "--temperature", "0", "--cache-dtype", "float8"]) == 0
     assert len(capsys.readouterr().out.strip().split(",")) == 6
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["gpt2", "dizizen"])
+def test_decoding_in_two_groups_side_by_side(name, dtype):
+    """40 sequences whose captured step takes its requests through the layers in two groups on two streams, against one group."""
+    config = {"gpt2": TINY_A, "dizizen": DIZIZEN["mixed"]}[name]
+    prompts = [random_tokens(300 + i, 21, config.get("vocab_size", config.get("vocab"))) for i in range(40)]
+    results = []
+    for lanes in (None, 32):
+        with engine_for(config, 5, dtype, max_sessions=40, page_size=16, decode_lanes_from=lanes) as engine:
+            handles = [engine.try_take_cache() for _ in prompts]
+            got = [[engine.prefill_greedy(h, p)] for h, p in zip(handles, prompts)]
+            engine.decode_batch_enqueue(handles)
+            for step in range(40):
+                if step < 39:
+                    engine.decode_batch_enqueue(handles)
+                for tokens, token in zip(got, engine.take()):
+                    tokens.append(token)
+            graph, = [g for key, g in engine.runner._graphs.items() if key[:2] == (64, True)]
+            assert (graph.lanes is not None) == (lanes is not None)
+            results.append(got)
+    assert results[0] == results[1]
