@@ -25,6 +25,14 @@ struct AttendArguments {
     float sink_factor;   // log2 e where weights are powers of two
 };
 
+// A head's sink among its scores, in their unit and finite; no score without sinks. It counts for their maximum as well: what a sink is above all
+// of them would not fit 32 bits as a weight.
+__device__ __forceinline__ float sink_score(const AttendArguments& a, int head) {
+    if (!a.sinks) return NO_SCORE;
+    const float sink = a.sinks[head] * a.sink_factor;
+    return sink > -NO_SCORE ? -NO_SCORE : sink;
+}
+
 // One result: of row `row`, element `at` of its n_heads * head_size.
 template <typename T>
 __device__ __forceinline__ void put_result(const AttendArguments& a, int row, int at, float value) {
@@ -118,18 +126,17 @@ __device__ __forceinline__ void attend_row(const AttendArguments& a, int row, in
     for (int i = threadIdx.x; i < columns * head_size; i += threads) {
         const int c = i / head_size, d = i % head_size;
         const float* const at = meeting + c * pitch;
-        float top = NO_SCORE;
+        const float sink = alone ? sink_score(a, head0 + c) : NO_SCORE;
+        float top = sink;
         for (int w = 0; w < waves; w++) top = fmaxf(top, at[w * columns * pitch + head_size]);
-        float total = 0.0f, value = 0.0f;
+        float total = alone && a.sinks ? weight_of<WIDE>(sink - top) : 0.0f, value = 0.0f;
         for (int w = 0; w < waves; w++) {
             const float factor = weight_of<WIDE>(at[w * columns * pitch + head_size] - top);
             total += at[w * columns * pitch + head_size + 1] * factor;
             value += at[w * columns * pitch + d] * factor;
         }
-        if (alone) {
-            if (a.sinks) total += weight_of<WIDE>(a.sinks[head0 + c] * a.sink_factor - top);
-            put_result<T>(a, row, (head0 + c) * head_size + d, value / total);
-        } else {
+        if (alone) put_result<T>(a, row, (head0 + c) * head_size + d, value / total);
+        else {
             float* const part = parts + (((size_t)row * a.n_heads + head0 + c) * n_runs + run) * (head_size + 2);
             part[d] = value;
             if (d == 0) {
@@ -207,10 +214,11 @@ __device__ __forceinline__ void attend_tile(const AttendArguments& a, int reques
         const int row = i / fours, d = 4 * (i % fours);
         if (row0 + row >= q_len) break;
         const int of_group = GROUPS == 1 ? 0 : row / WAVE_ROWS, at = GROUPS == 1 ? row : row % WAVE_ROWS;
-        float top = NO_SCORE;
+        const float sink = sink_score(a, head);
+        float top = sink;
 #pragma unroll
         for (int w = 0; w < SPLITS; w++) top = fmaxf(top, lds.meeting[w * GROUPS + of_group][at][HD]);
-        float total = a.sinks ? weight_of<WIDE>(a.sinks[head] * a.sink_factor - top) : 0.0f;
+        float total = a.sinks ? weight_of<WIDE>(sink - top) : 0.0f;
         f32x4 value = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < SPLITS; w++) {

@@ -32,7 +32,8 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(AttendArguments a, in
     const int pitch = head_size + 2;
     const float* const mine = parts + ((size_t)row * a.n_heads + head) * n_runs * pitch;
     float* const factor = factors + wave * n_runs;
-    float top = NO_SCORE;
+    const float sink = sink_score(a, head);
+    float top = sink;
     for (int r = lane; r < runs; r += WAVE) top = fmaxf(top, mine[r * pitch + head_size]);
     top = wave_max_total(top);
     float total = 0.0f;
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(256) void scaled_merge_kernel(AttendArguments a, in
         total += mine[r * pitch + head_size + 1] * f;
     }
     total = wave_total(total);
-    if (a.sinks) total += weight_of<WIDE>(a.sinks[head] * a.sink_factor - top);
+    if (a.sinks) total += weight_of<WIDE>(sink - top);
     __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");   // (the wave's own factors, by its other lanes)
     __builtin_amdgcn_wave_barrier();
     for (int d = lane; d < head_size; d += WAVE) {
