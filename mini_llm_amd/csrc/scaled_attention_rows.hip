@@ -7,8 +7,8 @@ namespace {
 constexpr int rows_waves(int padded, int size) { return padded == 64 ? (size == 2 ? 16 : 8) : 1024 / padded; }
 
 // A block per row, set of heads and run of keys. What bounds it is the cache's bytes, 2 (head_size + 0.25) a key for all
-// heads of a set together: 16 rows at 20,000 to 32,000 keys of 8 heads of 128 (32 query heads) 142 us for 810 MB, 5.7 TB/s; 64 rows of 0 to 1,023 keys of 12 heads of 64 13.4 us for
-// 51 MB, where the longest row is what is waited for; one row of 1,000 keys 7.1 us, a launch and four trips to memory.
+// heads of a set together: 16 rows at 20,000 to 32,000 keys of 8 heads of 128 (32 query heads) 142 us for 810 MB, 5.7 TB/s; 64 rows of 0 to 1,023 keys of 12 heads of 64 15.4 us for
+// 51 MB, where the longest row is what is waited for; one row of 1,000 keys 7.4 us, a launch and four trips to memory.
 template <typename T, int HD, bool WHOLE>
 __global__ __launch_bounds__(WAVE * rows_waves(HD, sizeof(T))) void scaled_rows_attention_kernel(AttendArguments a, int run_tiles, int n_runs, float* __restrict__ parts) {
     extern __shared__ float meeting[];

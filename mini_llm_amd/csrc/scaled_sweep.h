@@ -10,6 +10,11 @@
 //    (v_cvt_scalef32_pk_bf16_fp8: two numbers an instruction).
 //  * The running maximum of a column is raised only in a tile with a score more than 8 above it (weights up to 2^8, or e^8, in between):
 //    most tiles have no exchange between lanes and no rescaling at all.
+//  * Weights of a row by itself are two bfloat16 numbers, the second what the first leaves (2^-16 of the weight is lost), as over plain pages, where such rows
+//    keep them in 32 bits: memory is what bounds them. In one piece they took 7.0 for 7.4 us (one row of 1,000 keys), 14.3 for 15.4 (64 of up to 1,023), and
+//    as long for 16 of 20,000 and more, with results up to 32 times further off than two pieces allow before they are rounded. Weights of a portion's rows are rounded to bfloat16,
+//    2^-8 of each, as over plain pages: two pieces would be half as many products again on the matrix cores that bound them, 28.0 for 20.9 us (2,048 rows,
+//    12 heads of 64), 382 for 283 (8,191, 16 of 128). The sum that divides is of the weights as rounded.
 // WIDE (32-bit queries and results): queries and weights go through the products as three bfloat16 pieces that add up to them exactly, so
 // every product of a query or weight with a held number is exact in 32-bit.
 #pragma once
@@ -86,6 +91,7 @@ __device__ __forceinline__ float weight_of(float x) {
 template <int HD, int CT, bool WIDE, bool APART, bool WHOLE>
 struct ScaledSweep {
     static constexpr int NC = HD / 64, DT = HD / 16, NP = WIDE ? 3 : 1;
+    static constexpr int NW = WIDE ? 3 : APART ? 1 : 2;   // pieces of a weight
 
     // The queries' operands: rows of a portion, which all waves of a block share, in LDS ([CT][NC][2][NP][WAVE]); a row's heads in registers.
     bf16x8 q[APART ? 1 : CT][NC][2][NP];
@@ -117,9 +123,12 @@ struct ScaledSweep {
         }
     }
 
-    static __device__ __forceinline__ void in_pieces(float x, bf16_t (&piece)[NP]) {
-        if constexpr (!WIDE) piece[0] = static_cast<bf16_t>(x);
-        else {
+    template <int N>
+    static __device__ __forceinline__ void in_pieces(float x, bf16_t (&piece)[N]) {
+        if constexpr (N < 3) {
+            piece[0] = static_cast<bf16_t>(x);
+            if constexpr (N == 2) piece[1] = static_cast<bf16_t>(x - to_float(piece[0]));
+        } else {
             // the leading eight bits, the next eight, and the rest: cut off, not rounded, so that nothing overflows
             auto head_of = [](float y) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & 0xffff0000u); };
             const float a = head_of(x), r = __builtin_isinf(x) ? 0.0f : x - a, b = head_of(r);
@@ -319,7 +328,7 @@ struct ScaledSweep {
                     for (int i = 0; i < 4; i++) o[ct][dt][i] *= fall;
             }
         }
-        bf16x8 weights[CT][2][NP];
+        bf16x8 weights[CT][2][NW];
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             float sum = 0.0f;
@@ -329,10 +338,10 @@ struct ScaledSweep {
                 for (int i = 0; i < 4; i++) {
                     const float p = weight_of<WIDE>(__builtin_fmaf(s[ct][t][i], factor, -m[ct]));
                     if constexpr (WIDE) sum += p;
-                    bf16_t piece[NP];
+                    bf16_t piece[NW];
                     in_pieces(p, piece);
 #pragma unroll
-                    for (int n = 0; n < NP; n++) weights[ct][t / 2][n][4 * (t % 2) + i] = piece[n];
+                    for (int n = 0; n < NW; n++) weights[ct][t / 2][n][4 * (t % 2) + i] = piece[n];
                 }
             if constexpr (WIDE) l[ct] += sum;
         }
@@ -342,7 +351,9 @@ struct ScaledSweep {
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) l_rows[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, weights[ct][h][0], l_rows[ct], 0, 0, 0);
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int n = NW - 1; n >= 0; n--) l_rows[ct] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, weights[ct][h][n], l_rows[ct], 0, 0, 0);
         }
         if constexpr (MASKED) {
             // Not even a weight of zero silences a NaN: codes that are no number are taken out where no column sees them (places that nothing was
@@ -404,10 +415,10 @@ struct ScaledSweep {
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                for (int n = NP - 1; n >= 0; n--)
+                for (int n = NW - 1; n >= 0; n--)
                     o[ct][step / 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(values[step % 2], weights[ct][step % 2][n], o[ct][step / 2], 0, 0, 0);
             if constexpr (APART) {
-                interleave<1, CT * NP, 4>();
+                interleave<1, CT * NW, 4>();
                 if (step % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         }
