@@ -70,16 +70,14 @@ __device__ __forceinline__ bf16x8 eight_numbers(uint32_t lo, uint32_t hi, float 
 // The high bit of every byte of four codes that are no number (s1111111).
 __device__ __forceinline__ uint32_t not_numbers(uint32_t codes) { return ((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// Rows of a call that fall into one block: they are neighbours and their slots follow each other. Lane i of a wave looks at row `from` + i (32 of them are
-// enough: a run has at most 16 rows); the bits of the result are the rows that begin a run, rows behind the last among them. Rows
+// Rows of a call that fall into one block are a run where they are neighbours and their slots follow each other. Lane i of a wave looks at row `from` + i (32 of them are
+// enough: a run has at most 16 rows), whose slot is left in `slot`; the bits of the result are the rows that begin a run, rows behind the last among them. Rows
 // that go nowhere (their slots are negative, or lie behind the pages) are runs of their own, as many neighbours as up to the next multiple of 16.
-__device__ __forceinline__ uint32_t run_begins(const int* __restrict__ slots, int from, int n_rows, long long n_slots, int lane) {
-    const int row = from + (lane & 31);
-    bool begins = true;
-    if (row < n_rows && row > 0) {
-        const int slot = slots[row], before = slots[row - 1];
-        const bool nowhere = slot < 0 || slot >= n_slots, before_nowhere = before < 0 || before >= n_slots;
-        begins = nowhere != before_nowhere || (nowhere ? row % BLOCK_TOKENS == 0 : slot / BLOCK_TOKENS != before / BLOCK_TOKENS || slot != before + 1);
-    }
-    return (uint32_t)__ballot(begins);
+__device__ __forceinline__ uint32_t run_begins(const int* __restrict__ slots, int from, int n_rows, long long n_slots, int lane, int& slot) {
+    const int row = from + (lane & 31), here = min(row, n_rows - 1);
+    slot = slots[here];
+    const int before = slots[max(here - 1, 0)];
+    const bool nowhere = slot < 0 || slot >= n_slots, before_nowhere = before < 0 || before >= n_slots;
+    const bool follows = nowhere ? row % BLOCK_TOKENS != 0 : slot / BLOCK_TOKENS == before / BLOCK_TOKENS && slot == before + 1;
+    return (uint32_t)__ballot(row <= 0 || row >= n_rows || nowhere != before_nowhere || !follows);
 }

@@ -434,13 +434,149 @@ __device__ __forceinline__ void keys_by_elements(const AppendArguments& a, const
     if (lane == 0) a.k_scales[block] = two_to(scale.exponent);
 }
 
+// Where a call's rows go, shared among a block's 256 threads in pieces of four that lie on 16 bytes; the first 2,048 are on their way from the start.
+struct CallSlots {
+    const int* from;   // the first piece
+    int head, pieces, lone;
+    int4 held[2];
+    int lone_slot;     // a row in front of the pieces, or behind them
+    __device__ __forceinline__ CallSlots(const int* __restrict__ slots, int n_rows) {
+        head = min((int)(-(intptr_t)slots >> 2 & 3), n_rows);
+        from = slots + head;
+        pieces = (n_rows - head) / 4;
+        const int thread = threadIdx.x, behind = head + 4 * pieces + thread - 4;
+        lone = thread < 4 ? (thread < head ? thread : -1) : behind < n_rows ? behind : -1;
+        lone_slot = slots[max(lone, 0)];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (thread + 256 * i < pieces) held[i] = reinterpret_cast<const int4*>(from)[thread + 256 * i];
+    }
+    // Whether the calling thread's share has a row outside first .. first + count - 1 in the block of `slot`.
+    __device__ __forceinline__ bool elsewhere(int slot, int first, int count) const {
+        auto counts = [&](int row, int to) { return to >> 4 == slot >> 4 && (unsigned)(row - first) >= (unsigned)count; };
+        auto four = [&](int piece, int4 to) {
+            const int row = head + 4 * piece;
+            return counts(row, to.x) | counts(row + 1, to.y) | counts(row + 2, to.z) | counts(row + 3, to.w);
+        };
+        bool some = lone >= 0 && counts(lone, lone_slot);
+#pragma unroll
+        for (int i = 0; i < 2; i++) some |= (int)threadIdx.x + 256 * i < pieces && four(threadIdx.x + 256 * i, held[i]);
+#pragma unroll 4
+        for (int piece = threadIdx.x + 512; piece < pieces; piece += 256) some |= four(piece, reinterpret_cast<const int4*>(from)[piece]);
+        return some;
+    }
+};
+
+// Where a block's rows do not stand together, two blocks of threads would read and write its scale and rescale its codes at once: `runs_apart` finds such runs, and
+// append_apart takes them.
+//
+// Of the runs that begin in a block of threads' rows (bits of `begins`), those whose block has rows elsewhere in the call too. A run that fills its block leaves no
+// place for others, so that a prompt's are not asked. Calls of up to 256 rows are looked over by each wave.
+template <typename Elsewhere>
+__device__ __forceinline__ uint32_t runs_apart(const AppendArguments& a, uint32_t begins, int window, int per, int slot_here, bool& asked, const Elsewhere& elsewhere) {
+    uint32_t apart = 0;
+    while (begins) {
+        const int at = __builtin_ctz(begins), first = window + at;
+        if (at >= per || first >= a.n_rows) break;
+        begins &= begins - 1;
+        const int count = min((begins ? __builtin_ctz(begins) : 32) - at, a.n_rows - first), slot = __builtin_amdgcn_readlane(slot_here, at);
+        if (count == BLOCK_TOKENS || slot < 0 || slot >= a.n_slots) continue;
+        asked = true;
+        apart |= __any(elsewhere(slot, first, count)) ? 1u << at : 0u;
+    }
+    return apart;
+}
+
+// The row that goes to `slot`, the last of several; -1: none.
+__device__ __forceinline__ int row_of(const int* __restrict__ slots, int n_rows, int slot, int lane) {
+    int last = -1;
+    for (int row = lane; row < n_rows; row += WAVE) last = slots[row] == slot ? row : last;
+#pragma unroll
+    for (int step = 1; step < WAVE; step *= 2) last = max(last, __shfl_xor(last, step, WAVE));
+    return __builtin_amdgcn_readfirstlane(last);
+}
+
+// A token of a head's keys or values, by a wave, an element a lane.
+template <typename T, int E, bool KEYS>
+__device__ __forceinline__ void append_token(const AppendArguments& a, int row, size_t block, int token, int head, int lane) {
+    const int dim = KEYS ? a.dim : a.vdim;
+    const Turn& turn = KEYS ? a.turn : a.v_turn;
+    uint8_t* const codes = (KEYS ? a.k_codes : a.v_codes) + block * BLOCK_TOKENS * a.head_size;
+    float* const scales = KEYS ? a.k_scales : a.v_scales;
+    const T* const from = static_cast<const T*>(a.rows) + (size_t)row * a.stride + (KEYS ? a.k_at : a.v_at) + head * dim;
+    const bool normed = KEYS && (a.k_gain != nullptr || a.unit);
+    float x[E], sum = 0.0f, largest = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        x[e] = lane + e * WAVE < dim ? to_float(from[lane + e * WAVE]) : 0.0f;
+        sum += x[e] * x[e];
+    }
+    const float factor = normed ? rsqrtf(wave_total(sum) / (float)dim + a.eps) : 1.0f;
+    auto weighted = [&](float value, int d) { return normed ? value * (factor * (a.k_gain ? a.k_gain[d] : 1.0f)) : value; };
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int d = lane + e * WAVE;
+        if (d >= dim) continue;
+        x[e] = weighted(x[e], d);
+        if (turn.frequencies && d < turn.dims) {
+            int pair;
+            bool is_first;
+            const int other = partner_of(turn, d, pair, is_first);
+            double2 cs;
+            turn_of(a.positions[row], turn.frequencies[pair], cs.x, cs.y);
+            x[e] = turned_once(x[e], weighted(to_float(from[other]), other), is_first, cs);
+        }
+        largest = fmaxf(largest, counted_magnitude(x[e]));
+    }
+    const BlockScale scale(wave_max_total(largest), token, scales[block]);
+    if (KEYS) {
+        if (scale.grown) rescale_keys(codes, a.head_size, token, scale.factor, lane);
+    } else if (scale.grown)
+        for (int d = lane; d < a.head_size; d += WAVE)
+            for (int t = 0; t < token; t++) codes[d * BLOCK_TOKENS + t] = (uint8_t)rescaled_codes(codes[d * BLOCK_TOKENS + t], scale.factor);
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        const int d = lane + e * WAVE;
+        if (d < a.head_size)
+            codes[KEYS ? ((d / 16) * BLOCK_TOKENS + token) * 16 + d % 16 : d * BLOCK_TOKENS + token] = (uint8_t)four_codes(ready_for_code(x[e], scale.inverse), 0.0f, 0.0f, 0.0f);
+    }
+    if (lane == 0) scales[block] = two_to(scale.exponent);
+}
+
+// Blocks whose rows do not stand together, of the runs `apart`: who has a block's first row takes them all, one after another as their tokens are; a wave has a
+// head's, first_job and every step-th from there.
+template <typename T, int E>
+__device__ __forceinline__ void append_apart(const AppendArguments& a, uint32_t apart, int window, int first_job, int step, int lane) {
+    while (apart) {
+        const int first = window + __builtin_ctz(apart), slot = a.slots[first] & ~(BLOCK_TOKENS - 1);
+        apart &= apart - 1;
+        bool in_front = false;
+        for (int row = lane; row < first; row += WAVE) in_front |= (a.slots[row] & ~(BLOCK_TOKENS - 1)) == slot;
+        if (__any(in_front)) continue;
+        const size_t block = (((size_t)(slot >> a.page_shift) * a.n_kv_heads) << (a.page_shift - 4)) + ((slot & ((1 << a.page_shift) - 1)) / BLOCK_TOKENS);
+        for (int token = 0; token < BLOCK_TOKENS; token++) {
+            const int row = row_of(a.slots, a.n_rows, slot + token, lane);
+            if (row < 0) continue;
+            for (int job = first_job; job < 2 * a.n_kv_heads; job += step) {
+                const int head = job % a.n_kv_heads;
+                const size_t at = block + ((size_t)head << (a.page_shift - 4));
+                if (job < a.n_kv_heads) append_token<T, E, true>(a, row, at, token, head, lane);
+                else append_token<T, E, false>(a, row, at, token, head, lane);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");   // (what a lane has written is read by others of its wave for the next token)
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+}
+
 // A block of threads: a run of rows after another (those that begin in its rows: one each of the first `singles`, then `most`). The cosines and sines of the run's positions are made
 // once for all heads; then every wave takes heads: keys, values, queries.
 // A head of a run is one wave's, because a block has one scale: the largest magnitude is a reduction inside the wave, and what is held in front of the
 // new tokens is rounded again by who knows the new scale. Few rows: bound by the chain of dependent steps (slots, positions, cosines in 64-bit, rows, the block's scale, codes) behind
-// the launch, 5.2 us for one row of 12 heads of 64, 5.7 for 64 rows, 16 for 1,950 ragged ones (float32). Many rows: 8,192 of 32 + 16 heads of 128 (bfloat16, turned) 49 us, 168 MB read
-// and written at 3.4 TB/s (a large copy: 4.7); vector instructions are issued in half the cycles, the 64-bit turns of keys among them, and at three waves a SIMD the rest is not hidden behind
-// them. Asking for a wave's next head while it works on one takes the registers of the occupancy: 82 us for 72 with the read-back.
+// the launch, 5.2 us for one row of 12 heads of 64, 5.8 for 64 rows, 16.7 for 1,950 ragged ones (float32). Many rows: 8,192 of 32 + 16 heads of 128 (bfloat16, turned) 64 us, 185 MB
+// (168 of rows and queries, 17 of codes) at 2.9 TB/s (a large copy: 4.7); vector instructions are issued in half the cycles, the 64-bit turns of keys among them, and at three waves a SIMD the
+// rest is not hidden behind them. Asking for a wave's next head while it works on one takes the registers of the occupancy: 82 us for 72 with the read-back.
+// Looking for rows that do not stand together takes of these 0.3, 0.2, 0.8 and 3 us.
 template <typename T, int E, bool PIECES>
 __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_append_kernel(AppendArguments a, int singles, int most) {
     extern __shared__ double2 tables[];   // of queries and keys, of values, and of queries in 32 bits
@@ -448,8 +584,33 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
     const bool single = (int)blockIdx.x < singles;
     const int per = single ? 1 : most, window = single ? blockIdx.x : singles + ((int)blockIdx.x - singles) * most;
     const bool keeps = a.k_at >= 0;
-    // (queries alone have no blocks: any rows are a run)
-    uint32_t begins = keeps ? run_begins(a.slots, window, a.n_rows, a.n_slots, lane) : per == 1 ? 0xffffffffu : 0x00010001u;
+    uint32_t begins = per == 1 ? 0xffffffffu : 0x00010001u, apart = 0;   // (queries alone have no blocks: any rows are a run)
+    int slot_here = -1;   // of row window + lane
+    if (keeps) {
+        bool asked = false;
+        if (a.n_rows <= 4 * WAVE) {
+            int held[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) held[i] = a.slots[min(lane + WAVE * i, a.n_rows - 1)];
+            begins = run_begins(a.slots, window, a.n_rows, a.n_slots, lane, slot_here);
+            apart = runs_apart(a, begins, window, per, slot_here, asked, [&](int slot, int first, int count) {
+                bool some = false;
+#pragma unroll
+                for (int i = 0; i < 4; i++) some |= held[i] >> 4 == slot >> 4 && (unsigned)(min(lane + WAVE * i, a.n_rows - 1) - first) >= (unsigned)count;
+                return some;
+            });
+        } else {
+            __shared__ uint32_t met[4];
+            const CallSlots call(a.slots, a.n_rows);
+            begins = run_begins(a.slots, window, a.n_rows, a.n_slots, lane, slot_here);
+            apart = runs_apart(a, begins, window, per, slot_here, asked, [&](int slot, int first, int count) { return call.elsewhere(slot, first, count); });
+            if (asked) {
+                if (lane == 0) met[wave] = apart;
+                __syncthreads();
+                apart = __builtin_amdgcn_readfirstlane(met[0] | met[1] | met[2] | met[3]);
+            }
+        }
+    }
     const int pairs = a.turn.frequencies ? a.turn.dims / 2 : 0, v_pairs = a.v_turn.frequencies && keeps ? a.v_turn.dims / 2 : 0;
     double2* const wide = tables;
     double2* const v_wide = wide + BLOCK_TOKENS * turn_pitch(pairs);
@@ -460,10 +621,10 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
         const int at = __builtin_ctz(begins);
         Run run;
         run.first = window + at;
-        if (at >= per || run.first >= a.n_rows) return;
+        if (at >= per || run.first >= a.n_rows) break;
         begins &= begins - 1;
         run.count = __builtin_amdgcn_readfirstlane(min((begins ? __builtin_ctz(begins) : 32) - at, a.n_rows - run.first));   // at most 16
-        const int slot = keeps ? a.slots[run.first] : -1;
+        const int slot = __builtin_amdgcn_readlane(slot_here, at);
         run.kept = slot >= 0 && slot < a.n_slots;
         run.lead = slot & (BLOCK_TOKENS - 1);
         run.head_blocks = (size_t)1 << (a.page_shift - 4);
@@ -481,7 +642,7 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
             }
             __syncthreads();
         }
-        const int keys = run.kept ? a.n_kv_heads : 0;
+        const int keys = run.kept && !(apart >> at & 1) ? a.n_kv_heads : 0;
         const int queries = a.q_at < 0 ? 0 : PIECES ? a.n_heads : a.n_heads * run.count;
         for (int job = blockIdx.y * waves + wave; job < 2 * keys + queries; job += gridDim.y * waves) {
             int here = lane;
@@ -494,6 +655,11 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
             else query_by_elements<T, E>(a, run, (job - 2 * keys) / a.n_heads, (job - 2 * keys) % a.n_heads, turns, here);
         }
         if (pairs + v_pairs) __syncthreads();
+    }
+    if (apart) {
+        auto again = (const __attribute__((address_space(4))) AppendArguments*)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(again));   // (the arguments read again: kept for a path that is hardly ever taken, they take the registers of the others)
+        append_apart<T, E>(*(const AppendArguments*)again, apart, window, blockIdx.y * 4 + threadIdx.x / WAVE, gridDim.y * 4, lane);
     }
 }
 
@@ -514,13 +680,14 @@ __global__ __launch_bounds__(256) void scaled_rows_kernel(const uint8_t* __restr
     const int window = blockIdx.x * per, head = blockIdx.y * 4 + wave;
     if (head >= n_kv_heads) return;
     const size_t row_size = (size_t)n_kv_heads * head_size;
-    uint32_t begins = run_begins(slots, window, n_rows, n_slots, lane);
+    int slot_here;
+    uint32_t begins = run_begins(slots, window, n_rows, n_slots, lane, slot_here);
     while (begins) {
         const int at = __builtin_ctz(begins), first = window + at;
         if (at >= per || first >= n_rows) return;
         begins &= begins - 1;
         const int count = min((begins ? __builtin_ctz(begins) : 32) - at, n_rows - first);
-        const int slot = slots[first];
+        const int slot = __builtin_amdgcn_readlane(slot_here, at);
         T* const k_to = k_out + (size_t)first * row_size + head * head_size;
         T* const v_to = v_out + (size_t)first * row_size + head * head_size;
         if (slot < 0 || slot >= n_slots) {

@@ -1591,10 +1591,11 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     first ``rot_dims`` elements turn in pairs by position * frequencies[pair] (float64, the angle in 64-bit), pairs (i, i + rot_dims / 2) with ``pairing``
     "half" or (2i, 2i + 1) with "neighbours"; ``v_frequencies``, ``v_rot_dims`` and ``v_pairing`` turn the values likewise.
 
-    Keys and values of row r go to slots[r] = page * page_size + offset (negative, or behind the pages: nowhere). Rows whose slots fall into
-    one block are neighbours and follow each other, as a request's tokens do, and no slot is named twice. A block whose first token
-    is written begins afresh; a block that is carried on keeps its scale or, if the new rows need a larger one, is taken to that (its earlier
-    tokens' codes rounded again). Tokens of a block behind those written stay as they are. ``short_rows``: the first so many rows are of many requests
+    Keys and values of row r go to slots[r] = page * page_size + offset (negative, or behind the pages: nowhere), and no slot is named twice. Rows that
+    fall into one block and are neighbours whose slots follow each other, as a request's tokens are, are appended at once; where a block's rows do not stand
+    together, its tokens are appended one after another, the lowest first. A block whose first token is written begins afresh; a block that is carried
+    on keeps its scale or, if the new rows need a larger one, is taken to that (its earlier tokens' codes rounded again). The codes of a block's tokens
+    behind those written stay as they are (they count by the block's scale, whatever it becomes). ``short_rows``: the first so many rows are of many requests
     (as ``paged_attention`` has them); it says how the work is best cut and changes no result.
 
     Returns the queries [rows, n_heads * head_size] of ``out_dtype`` (default: the rows' type), zeros behind their ``dim`` elements (None without ``q_at``)."""
