@@ -1573,7 +1573,7 @@ def _strided_rows(t, name: str, width: int, here: int) -> int:
 def _rotation(frequencies, dims: int, most: int, pairing: str, name: str, here: int):
     """(address, turned elements) of a rotation, (None, 0) of none."""
     _require(pairing in ("half", "neighbours"), f"{name} pair by halves or by neighbours")
-    if frequencies is None or not dims:
+    if not dims:
         return None, 0
     dims = int(dims)
     _device_tensor(frequencies, f"the frequencies of {name}", torch.float64, 1)
