@@ -34,7 +34,7 @@ struct AppendArguments {
     uint8_t* v_codes;
     float* v_scales;
     long long n_slots;
-    int n_rows, n_heads, n_kv_heads, dim, vdim, head_size, page_shift, q_wide;
+    int n_rows, n_heads, n_kv_heads, dim, vdim, head_size, page_shift, q_wide, together;
 };
 
 // cos and sin of position x frequency to the last bits of 64: the turns are taken off in quarters, and what is left, at most pi / 4, goes
@@ -471,7 +471,7 @@ struct CallSlots {
 // append_apart takes them.
 //
 // Of the runs that begin in a block of threads' rows (bits of `begins`), those whose block has rows elsewhere in the call too. A run that fills its block leaves no
-// place for others, so that a prompt's are not asked. Calls of up to 256 rows are looked over by each wave.
+// place for others, so that a prompt's are not asked. Calls of up to 256 rows are looked over by each wave. A caller whose rows stand together can say so.
 template <typename Elsewhere>
 __device__ __forceinline__ uint32_t runs_apart(const AppendArguments& a, uint32_t begins, int window, int per, int slot_here, bool& asked, const Elsewhere& elsewhere) {
     uint32_t apart = 0;
@@ -588,7 +588,8 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
     int slot_here = -1;   // of row window + lane
     if (keeps) {
         bool asked = false;
-        if (a.n_rows <= 4 * WAVE) {
+        if (a.together) begins = run_begins(a.slots, window, a.n_rows, a.n_slots, lane, slot_here);
+        else if (a.n_rows <= 4 * WAVE) {
             int held[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) held[i] = a.slots[min(lane + WAVE * i, a.n_rows - 1)];
@@ -747,7 +748,7 @@ int shift_of(int page_size) {
 MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, int k_at, int v_at, const float* q_gain, const float* k_gain, float eps, int unit,
                                 const double* frequencies, int rot_dims, int neighbours, const double* v_frequencies, int v_rot_dims, int v_neighbours,
                                 const int* positions, const int* slots, void* q_out, void* k_codes, float* k_scales, void* v_codes, float* v_scales, int num_pages,
-                                int n_rows, int n_heads, int n_kv_heads, int dim, int vdim, int head_size, int page_size, int dtype, int q_dtype, int short_rows,
+                                int n_rows, int n_heads, int n_kv_heads, int dim, int vdim, int head_size, int page_size, int dtype, int q_dtype, int short_rows, int together,
                                 hipStream_t stream) {
     MLLM_REQUIRE(n_rows >= 0 && n_heads > 0 && n_kv_heads > 0 && num_pages > 0, "scaled_append: bad sizes");
     MLLM_REQUIRE(head_size > 0 && head_size % 16 == 0 && head_size <= SCALED_MAX_HEAD && dim > 0 && dim <= head_size && vdim > 0 && vdim <= head_size,
@@ -764,7 +765,7 @@ MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, in
                  "scaled_append: a missing operand");
     AppendArguments a = {rows, stride, q_at, k_at, v_at, q_gain, k_gain, eps, unit, {rot_dims ? frequencies : nullptr, rot_dims, neighbours},
                          {v_rot_dims ? v_frequencies : nullptr, v_rot_dims, v_neighbours}, positions, slots, q_out, (uint8_t*)k_codes, k_scales, (uint8_t*)v_codes, v_scales,
-                         (long long)num_pages * page_size, n_rows, n_heads, n_kv_heads, dim, vdim, head_size, shift_of(page_size), q_dtype == MLLM_F32};
+                         (long long)num_pages * page_size, n_rows, n_heads, n_kv_heads, dim, vdim, head_size, shift_of(page_size), q_dtype == MLLM_F32, together};
     // pieces of eight elements: everything lies on 16 bytes, and what turns with each other lies in whole pieces
     const int size = dtype == MLLM_F32 ? 4 : 2;
     const bool on_pieces = (uintptr_t)rows % 16 == 0 && stride * size % 16 == 0 && dim % 16 == 0 && rot_dims % 16 == 0 && (q_at < 0 || (q_at * size % 16 == 0 && (uintptr_t)q_out % 16 == 0)) &&

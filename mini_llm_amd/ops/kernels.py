@@ -1584,7 +1584,7 @@ def _rotation(frequencies, dims: int, most: int, pairing: str, name: str, here: 
 
 def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_pages, v_pages, slots, positions, n_heads: int, n_kv_heads: int, dim: int, vdim: int, *, q_gain=None,
                   k_gain=None, unit: bool = False, eps: float = 0.0, frequencies=None, rot_dims: int = 0, pairing: str = "half", v_frequencies=None, v_rot_dims: int = 0,
-                  v_pairing: str = "half", out_dtype=None, short_rows: int = 0):
+                  v_pairing: str = "half", out_dtype=None, short_rows: int = 0, together: bool = False):
     """The row-wise work between a mixer's input product and its attention over pages of 8 bits (``ScaledPages``), in one kernel. ``rows``
     (float32 or bfloat16; rows may be strided): the queries [n_heads, dim] at column ``q_at`` (None: no queries are made), the keys [n_kv_heads, dim]
     at ``k_at`` and the values [n_kv_heads, vdim] at ``v_at`` (both None: the layer reads pages another layer keeps, and only its queries are
@@ -1597,7 +1597,8 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     together, its tokens are appended one after another, the lowest first. A block whose first token is written begins afresh; a block that is carried
     on keeps its scale or, if the new rows need a larger one, is taken to that (its earlier tokens' codes rounded again). The codes of a block's tokens
     behind those written stay as they are (they count by the block's scale, whatever it becomes). ``short_rows``: the first so many rows are of many requests
-    (as ``paged_attention`` has them); it says how the work is best cut and changes no result.
+    (as ``paged_attention`` has them); it says how the work is best cut and changes no result. ``together``: the caller's word that every block's rows do stand
+    together, as those of the engine's steps do; nothing is looked for then (0.2 to 3 us), and where it is not so what such blocks hold is undefined.
 
     Returns the queries [rows, n_heads * head_size] of ``out_dtype`` (default: the rows' type), zeros behind their ``dim`` elements (None without ``q_at``)."""
     num_pages, _, page_size, head_size = k_pages.shape
@@ -1625,7 +1626,7 @@ def scaled_append(rows, q_at: int | None, k_at: int | None, v_at: int | None, k_
     q = rows.new_empty((n, n_heads * head_size), dtype=out_dtype) if makes else None
     check(library().mllm_scaled_append(rows.data_ptr(), stride, q_at if makes else -1, k_at if keeps else -1, v_at if keeps else -1, q_gain, k_gain, eps, bool(unit), frequencies,
                                        rot_dims, pairing == "neighbours", v_frequencies, v_rot_dims, v_pairing == "neighbours", position_at, slot_at, _ptr(q), *k_pages.addresses,
-                                       *v_pages.addresses, num_pages, n, n_heads, n_kv_heads, dim, vdim, head_size, page_size, _code(rows.dtype), _code(out_dtype), int(short_rows), _stream()))
+                                       *v_pages.addresses, num_pages, n, n_heads, n_kv_heads, dim, vdim, head_size, page_size, _code(rows.dtype), _code(out_dtype), int(short_rows), bool(together), _stream()))
     return q
 
 

@@ -112,7 +112,7 @@ _SIGNATURES = {
     "mllm_recurrence": [c_int, P, c_int, P, c_int, P, c_int, P, P, c_int, c_float, P, c_float, P, c_longlong, c_longlong, c_longlong, P, P, P, c_int, c_int,
                         c_int, c_int, c_int, P],
     "mllm_scaled_append": [P, c_longlong, c_int, c_int, c_int, P, P, c_float, c_int, P, c_int, c_int, P, c_int, c_int, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int,
-                           c_int, c_int, c_int, c_int, c_int, c_int, P],
+                           c_int, c_int, c_int, c_int, c_int, c_int, c_int, P],
     "mllm_scaled_rows": [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, P],
     "mllm_scaled_attention_rows": [P, c_longlong, P, P, P, P, P, c_longlong, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_float, P,
                                    c_int, c_int, c_int, c_int, c_int, c_int, c_int, P, P],

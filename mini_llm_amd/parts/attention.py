@@ -72,7 +72,7 @@ class CausalSelfAttention(Mixer):
             if isinstance(ctx.k_pages, kernels.ScaledPages):
                 if ctx.write_cache:
                     kernels.scaled_append(qkv, None, self.q_width, self.q_width + self.kv_width, ctx.k_pages, ctx.v_pages, ctx.group.slots, ctx.batch.positions,
-                                          self.n_heads, self.n_kv_heads, self.head_size, self.head_size, short_rows=ctx.batch.short_rows)
+                                          self.n_heads, self.n_kv_heads, self.head_size, self.head_size, short_rows=ctx.batch.short_rows, together=True)
             elif ctx.write_cache:
                 k = qkv[:, self.q_width : self.q_width + self.kv_width]
                 v = qkv[:, self.q_width + self.kv_width :]

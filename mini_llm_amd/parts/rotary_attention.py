@@ -150,7 +150,7 @@ class RotaryAttention(Mixer):
                                       q_gain=self.q_norm, k_gain=self.k_norm, unit=self.qk_norm == "unit", eps=self.eps,
                                       frequencies=None if rotary is None else rotary.frequencies64(x.device), rot_dims=0 if rotary is None else rotary.dims,
                                       v_frequencies=turn.frequencies64(x.device) if turn_dims else None, v_rot_dims=turn_dims,
-                                      v_pairing="half" if turn is None else turn.pairing, out_dtype=x.dtype, short_rows=batch.short_rows)
+                                      v_pairing="half" if turn is None else turn.pairing, out_dtype=x.dtype, short_rows=batch.short_rows, together=True)
         else:
             q = kernels.map_rows(fused, 0, k_at, v_at, self.q_norm, self.k_norm, self.eps, None if rotary is None else rotary.frequencies64(x.device),
                                  0 if rotary is None else rotary.dims, batch.positions, ctx.group.slots, ctx.k_pages, ctx.v_pages, self.n_heads,

@@ -152,3 +152,18 @@ def test_a_row_apart_in_a_captured_call():
             K.scaled_append(rows[i], None, 0, size, *wanted, ints(order), ints(order), 1, 1, size, size)
             for a, b in zip(pages, wanted):   # (every block is begun afresh)
                 assert torch.equal(a.codes.view(torch.uint8)[0], b.codes.view(torch.uint8)[0]) and torch.equal(a.scales[0], b.scales[0])
+
+
+@pytest.mark.parametrize("starts,counts", [([0, 9, 40, 31], [20, 1, 30, 2]), ([5, 0], [170, 200])], ids=["some", "many"])
+def test_a_caller_that_says_so_gets_the_same(starts, counts):
+    heads, size, n = 3, 64, sum(counts)
+    own, planes = prepared(starts, counts, 32, heads, size, n)
+    rows = torch.randn((n, 2 * heads * size), generator=torch.Generator().manual_seed(n)) * torch.exp(torch.randn((n, 1), generator=torch.Generator().manual_seed(2)))
+    slots = torch.tensor(own, dtype=torch.int32, device=DEVICE)
+    results = []
+    for together in (False, True):
+        pages = pages_of(planes)
+        kernels().scaled_append(rows.to(DEVICE), None, 0, heads * size, *pages, slots, slots, heads, heads, size, size, together=together)
+        results.append(pages)
+    for a, b in zip(*results):
+        assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.scales, b.scales)
