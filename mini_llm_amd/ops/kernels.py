@@ -1485,7 +1485,7 @@ class ScaledPages:
     ``codes`` (float8_e4m3fn): keys [num_pages, n_kv_heads, page_size / 16, head_size / 16, 16 tokens, 16 elements], values [num_pages,
     n_kv_heads, page_size / 16, head_size, 16 tokens]: a block lies as the matrix instructions take it (csrc/scaled_blocks.h). ``scales``:
     float32 [num_pages, n_kv_heads, page_size / 16]. ``scaled_append`` writes them, ``paged_attention`` reads them where it is given them as
-    pages, ``scaled_rows`` gives what they hold. Pages are the memory that the two tensors have when they are made. ``shape`` ([num_pages, n_kv_heads, page_size, head_size]) and ``dtype`` are as pages of plain
+    pages, ``scaled_rows`` gives what they hold. Pages go with the memory that the two tensors have when they are made. ``shape`` ([num_pages, n_kv_heads, page_size, head_size]) and ``dtype`` are as pages of plain
     rows have them."""
 
     __slots__ = ("codes", "scales", "shape", "is_keys", "on_gpu", "device_index", "addresses")
@@ -1507,9 +1507,8 @@ class ScaledPages:
         page_size, head_size = blocks * SCALE_BLOCK, of_codes[3] * 16 if keys else of_codes[3]
         if not (num_pages > 0 and n_kv_heads > 0 and blocks > 0 and blocks & (blocks - 1) == 0 and head_size % 16 == 0 and 0 < head_size <= SCALED_MAX_HEAD):
             raise OperandError(f"pages of {page_size} tokens (a power of two of at least {SCALE_BLOCK}) for heads of {head_size} (a multiple of 16 up to {SCALED_MAX_HEAD})")
-        # (tensors of its own over the same memory: that stays as it was looked at, whatever the caller's tensors are made to be later)
-        self.codes, self.scales, self.on_gpu = codes.detach(), scales.detach(), self.device_index >= 0
-        self.shape, self.addresses = (num_pages, n_kv_heads, page_size, head_size), (self.codes.data_ptr(), self.scales.data_ptr())
+        self.codes, self.scales, self.on_gpu = codes, scales, self.device_index >= 0
+        self.shape, self.addresses = (num_pages, n_kv_heads, page_size, head_size), (codes.data_ptr(), scales.data_ptr())
 
     @property
     def device(self):
@@ -1532,6 +1531,9 @@ def _check_scaled(k_pages, v_pages, n_kv_heads: int, head_size: int):
     shape = k_pages.shape
     _require(shape == v_pages.shape, "key and value pages differ in shape")
     _require(shape[1] == n_kv_heads and shape[3] == head_size, "pages do not match the heads")
+    (k_codes, k_scales), (v_codes, v_scales) = k_pages.addresses, v_pages.addresses
+    if k_pages.codes.data_ptr() != k_codes or k_pages.scales.data_ptr() != k_scales or v_pages.codes.data_ptr() != v_codes or v_pages.scales.data_ptr() != v_scales:
+        raise OperandError("the codes or the scales of these pages have been given other memory since the pages were made")
     _require(k_pages.on_gpu and v_pages.on_gpu, "the pages are not on the GPU: there is no CPU path")
     here = torch.cuda.current_device()   # kernels run on the current device's stream: what they are given lies there
     if k_pages.device_index != here or v_pages.device_index != here:

@@ -1,7 +1,5 @@
 """What pages of 8 bits are made of, and stay."""
 
-import gc
-
 import pytest
 import torch
 
@@ -9,18 +7,36 @@ from mini_llm_amd.ops import kernels as K
 
 
 @pytest.mark.parametrize("keys", [True, False])
-def test_pages_keep_their_memory_when_the_callers_tensors_become_others(keys):
-    codes = torch.zeros((3, 2, 4, 1, 16, 16) if keys else (3, 2, 4, 16, 16), dtype=torch.uint8).view(K.E4M3)
-    scales = torch.ones((3, 2, 4))
-    pages, at = K.ScaledPages(codes, scales), (codes.data_ptr(), scales.data_ptr())
-    scales[1, 0, 2] = 4.0
-    assert pages.scales[1, 0, 2] == 4.0
-    codes.data = torch.ones((1, 1), dtype=torch.uint8).view(K.E4M3)
-    scales.set_(torch.zeros(2))
-    del codes, scales
-    gc.collect()
-    assert pages.addresses == at == (pages.codes.data_ptr(), pages.scales.data_ptr())
-    assert pages.codes.numel() == 3 * 2 * 64 * 16 and pages.scales.shape == (3, 2, 4) and pages.scales[1, 0, 2] == 4.0 and not bool(pages.codes.view(torch.uint8).any())
+@pytest.mark.parametrize("which", ["codes", "scales"])
+@pytest.mark.parametrize("how", ["data", "set"])
+def test_pages_whose_tensors_have_other_memory_are_refused(keys, which, how):
+    k, v = K.scaled_pages(3, 2, 64, 16, "cpu")
+    pages, ints = k if keys else v, torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(K.OperandError, match="GPU"):
+        K.scaled_rows(k, v, ints)
+    tensor = pages.codes if which == "codes" else pages.scales
+    other = tensor[:1].clone()
+    if how == "data":
+        tensor.data = other
+    else:
+        tensor.set_(other)
+    for call in (lambda: K.scaled_rows(k, v, ints), lambda: K.scaled_append(torch.zeros((1, 96)), 0, 32, 64, k, v, ints, ints, 2, 2, 16, 16),
+                 lambda: K.paged_attention(torch.zeros((1, 32)), k, v, ints, ints, ints[None], 2, 2, 16, 0.25)):
+        with pytest.raises(K.OperandError, match="other memory"):
+            call()
+
+
+@pytest.mark.gpu
+def test_calls_over_pages_whose_tensors_have_other_memory_are_refused():
+    k, v = K.scaled_pages(4, 1, 16, 16, "cuda:0")
+    ints = torch.zeros(1, dtype=torch.int32, device="cuda:0")
+    rows = torch.ones((1, 48), device="cuda:0")
+    K.scaled_append(rows, 0, 16, 32, k, v, ints, ints, 1, 1, 16, 16)
+    v.codes.data = v.codes[:1].clone()
+    for call in (lambda: K.scaled_append(rows, 0, 16, 32, k, v, ints, ints, 1, 1, 16, 16), lambda: K.scaled_rows(k, v, ints),
+                 lambda: K.paged_attention(rows[:, :16], k, v, ints, ints, ints[None], 1, 1, 16, 0.25)):
+        with pytest.raises(K.OperandError, match="other memory"):
+            call()
 
 
 def test_a_rotation_without_frequencies_is_refused():
