@@ -487,15 +487,6 @@ __device__ __forceinline__ uint32_t runs_apart(const AppendArguments& a, uint32_
     return apart;
 }
 
-// The row that goes to `slot`, the last of several; -1: none.
-__device__ __forceinline__ int row_of(const int* __restrict__ slots, int n_rows, int slot, int lane) {
-    int last = -1;
-    for (int row = lane; row < n_rows; row += WAVE) last = slots[row] == slot ? row : last;
-#pragma unroll
-    for (int step = 1; step < WAVE; step *= 2) last = max(last, __shfl_xor(last, step, WAVE));
-    return __builtin_amdgcn_readfirstlane(last);
-}
-
 // A token of a head's keys or values, by a wave, an element a lane.
 template <typename T, int E, bool KEYS>
 __device__ __forceinline__ void append_token(const AppendArguments& a, int row, size_t block, int token, int head, int lane) {
@@ -546,16 +537,32 @@ __device__ __forceinline__ void append_token(const AppendArguments& a, int row, 
 // Blocks whose rows do not stand together, of the runs `apart`: who has a block's first row takes them all, one after another as their tokens are; a wave has a
 // head's, first_job and every step-th from there.
 template <typename T, int E>
-__device__ __forceinline__ void append_apart(const AppendArguments& a, uint32_t apart, int window, int first_job, int step, int lane) {
+__device__ __forceinline__ void append_apart(const AppendArguments& a, uint32_t apart, int window, int wave, int first_job, int step, int lane) {
+    __shared__ int rows_of[4][BLOCK_TOKENS];   // of a block's tokens, as each wave has found them
+    int* const mine = rows_of[wave];
+    auto settled = [] {   // what lanes have written is read by others of their wave
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");
+        __builtin_amdgcn_wave_barrier();
+    };
     while (apart) {
         const int first = window + __builtin_ctz(apart), slot = a.slots[first] & ~(BLOCK_TOKENS - 1);
         apart &= apart - 1;
+        if (lane < BLOCK_TOKENS) mine[lane] = -1;
+        settled();
         bool in_front = false;
-        for (int row = lane; row < first; row += WAVE) in_front |= (a.slots[row] & ~(BLOCK_TOKENS - 1)) == slot;
+#pragma unroll 8
+        for (int row = lane; row < a.n_rows; row += WAVE) {
+            const int to = a.slots[row];
+            if ((to & ~(BLOCK_TOKENS - 1)) == slot) {
+                atomicMax(&mine[to & (BLOCK_TOKENS - 1)], row);
+                in_front |= row < first;
+            }
+        }
+        settled();
         if (__any(in_front)) continue;
         const size_t block = (((size_t)(slot >> a.page_shift) * a.n_kv_heads) << (a.page_shift - 4)) + ((slot & ((1 << a.page_shift) - 1)) / BLOCK_TOKENS);
         for (int token = 0; token < BLOCK_TOKENS; token++) {
-            const int row = row_of(a.slots, a.n_rows, slot + token, lane);
+            const int row = __builtin_amdgcn_readfirstlane(mine[token]);
             if (row < 0) continue;
             for (int job = first_job; job < 2 * a.n_kv_heads; job += step) {
                 const int head = job % a.n_kv_heads;
@@ -563,8 +570,7 @@ __device__ __forceinline__ void append_apart(const AppendArguments& a, uint32_t 
                 if (job < a.n_kv_heads) append_token<T, E, true>(a, row, at, token, head, lane);
                 else append_token<T, E, false>(a, row, at, token, head, lane);
             }
-            __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "workgroup");   // (what a lane has written is read by others of its wave for the next token)
-            __builtin_amdgcn_wave_barrier();
+            settled();
         }
     }
 }
@@ -660,7 +666,7 @@ __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_appen
     if (apart) {
         auto again = (const __attribute__((address_space(4))) AppendArguments*)__builtin_amdgcn_kernarg_segment_ptr();
         asm volatile("" : "+s"(again));   // (the arguments read again: kept for a path that is hardly ever taken, they take the registers of the others)
-        append_apart<T, E>(*(const AppendArguments*)again, apart, window, blockIdx.y * 4 + threadIdx.x / WAVE, gridDim.y * 4, lane);
+        append_apart<T, E>(*(const AppendArguments*)again, apart, window, wave, blockIdx.y * 4 + wave, gridDim.y * 4, lane);
     }
 }
 
