@@ -6,9 +6,10 @@
 namespace {
 
 // A block per (request, head, tile of rows). Tiles with the most keys of all heads come first. What bounds it: a wave issues its own conversions, softmax
-// arithmetic and products one behind the other, and two waves a SIMD (what 250 registers leave) overlap in part: 16 heads of 128 on 8,192 rows 286 us, 961 TFLOP/s
-// of the keys that are seen (vector instructions in half the cycles, matrix instructions in a third); without the exponentials it would be 5 % less, without the reads of keys and values 22 %. 12 heads of 64 on 2,048
-// rows 20 us, where the launch is one round of blocks and the longest has eight tiles of keys a wave.
+// arithmetic and products one behind the other, and two waves a SIMD (what 250 registers leave) overlap in part: 16 heads of 128 on 8,192 rows (64 a block, two waves on each half) 281 us, 980 TFLOP/s
+// of the keys that are seen (vector instructions in half the cycles, matrix instructions in 46 %); without the exponentials it would be 2 to 5 % less, without the reads of keys and values 23 %.
+// 12 heads of 64 on 2,048 rows 21 us, where the launch is one round of blocks and the longest has eight tiles of keys a wave (without the exponentials 19.7, without the reads 20.1); this form, 64 rows
+// of heads of up to 64, takes all 256 registers and spills 5 (27 over pages of 16 or 32 tokens).
 template <typename T, int HD, int CT, int SPLITS, bool WHOLE>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void scaled_tiles_attention_kernel(AttendArguments a) {
     __shared__ TileMemory<T, HD, CT, SPLITS> lds;

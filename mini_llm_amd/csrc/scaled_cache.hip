@@ -38,8 +38,9 @@ struct AppendArguments {
 };
 
 // cos and sin of position x frequency to the last bits of 64: the turns are taken off in quarters, and what is left, at most pi / 4, goes
-// through the series of both (the first term left out is below 1e-16). Keys are rounded to 8 bits once, from 64: a key that lies
-// next to a border falls on the side where the exact one does.
+// through the series of both (the first term left out is below 1e-16). Keys and values that no norm
+// has rounded are rounded to 8 bits once, from 64: a number next to a border falls on the side where the exact one does. (A norm is taken in 32 bits, and a key out of it may fall to the
+// other side of a border that it lies next to: one code's step in few places.)
 __device__ __forceinline__ void turn_of(int position, double frequency, double& c, double& s) {
     const double angle = (double)position * frequency;
     const double quarters = rint(angle * 0.63661977236758134308);
@@ -579,10 +580,10 @@ __device__ __forceinline__ void append_apart(const AppendArguments& a, uint32_t 
 // once for all heads; then every wave takes heads: keys, values, queries.
 // A head of a run is one wave's, because a block has one scale: the largest magnitude is a reduction inside the wave, and what is held in front of the
 // new tokens is rounded again by who knows the new scale. Few rows: bound by the chain of dependent steps (slots, positions, cosines in 64-bit, rows, the block's scale, codes) behind
-// the launch, 5.2 us for one row of 12 heads of 64, 5.8 for 64 rows, 16.7 for 1,950 ragged ones (float32). Many rows: 8,192 of 32 + 16 heads of 128 (bfloat16, turned) 64 us, 185 MB
-// (168 of rows and queries, 17 of codes) at 2.9 TB/s (a large copy: 4.7); vector instructions are issued in half the cycles, the 64-bit turns of keys among them, and at three waves a SIMD the
-// rest is not hidden behind them. Asking for a wave's next head while it works on one takes the registers of the occupancy: 82 us for 72 with the read-back.
-// Looking for rows that do not stand together takes of these 0.3, 0.2, 0.8 and 3 us.
+// the launch, 5.2 us for one row of 12 heads of 64, 5.8 for 64 rows, 16.7 for 1,950 ragged ones (float32). Many rows: 8,192 of 32 + 16 heads of 128 (bfloat16, turned) 64 us in a row of such
+// calls, 54 by itself, 185 MB (168 of rows and queries, 17 of codes) at 2.9 and 3.4 TB/s (a large copy: 4.7); vector instructions are issued in six of ten cycles, the 64-bit turns of keys among
+// them, and at three waves a SIMD the rest is not hidden behind them: 168 registers do not hold one body's three kinds of heads (16 of a lane and 172 of a wave are spilled). Asking for a
+// wave's next head while it works on one takes more of them: 82 us for 72 with the read-back. Looking for rows that do not stand together takes 0.3, 0.2, 0.8 and 3 us of these.
 template <typename T, int E, bool PIECES>
 __global__ __launch_bounds__(256, E == 1 ? 4 : E == 2 ? 3 : 1) void scaled_append_kernel(AppendArguments a, int singles, int most) {
     extern __shared__ double2 tables[];   // of queries and keys, of values, and of queries in 32 bits
@@ -778,7 +779,7 @@ MLLM_API int mllm_scaled_append(const void* rows, long long stride, int q_at, in
                            (k_at < 0 || k_at * size % 16 == 0);
     // many rows: 16 to a block of threads, which finds the runs among them; few, or those that the caller says are of many requests: a block each, so that each
     // is under way at once. 32 rows of as many requests in front of 2,016 of a prompt, keys and values of 16 heads of 64, us without / with being told: 53 / 8.8
-    // (2,048 of a prompt alone 7.0); 512 single rows 32.5 / 15.6; 32 and 480 of 32 + 16 heads of 128, turned, with queries 75 / 11.3. Queries
+    // (2,048 of a prompt alone 7.0); 512 single rows 34.1 / 15.5; 32 and 480 of 32 + 16 heads of 128, turned, with queries 78 / 11.9 (rows said to stand together). Queries
     // alone, 32 heads of 128 turned, us with one row / 16 a block: 32 rows 5.5 / 6.4, 64 6.0 / 6.4, 128 9.4 / 6.5, 8,192 202 / 32.6.
     const int per = n_rows >= (k_at >= 0 ? 256 : 96) ? BLOCK_TOKENS : 1;
     const int singles = per == 1 || k_at < 0 ? 0 : std::max(0, std::min(short_rows, n_rows));

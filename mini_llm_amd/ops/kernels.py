@@ -1656,14 +1656,14 @@ def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int, wide: bool
     most = (8 if wide else 16) if head_size <= 64 else 8 if head_size <= 128 else 4   # (what the registers leave)
     while most > 1 and most * columns * (head_size + 4) * 4 > 65536:   # and what the LDS holds of their results
         most //= 2
-    # Rows of few tiles and launches of many blocks are not cut: putting runs together is another launch. us of 12 blocks of 16 tiles in 1 / 4 / 8 runs 7.5 / 9.0 /
-    # 9.0; of 200 of 15 (32-bit) in 1 / 3 / 5 11.1 / 14.3 / 13.6; of 768 of 63 in 1 / 3 / 5 60 / 64 / 65. Others are cut until there are two blocks for each of
-    # 256 compute units, into at most about sqrt(tiles) runs: of 12 of 63 in 3 / 5 / 9 / 21 11.0 / 9.9 / 9.9 / 10.4; of 8 of 469 (heads of 128) in 5 / 9 / 17 / 34 / 59
-    # 33 / 24 / 22 / 28 / 32; of 96 of 63 (32-bit) in 1 / 5 / 9 / 21 22.2 / 18.6 / 19.4 / 19.4; of 128 of 480 in 2 / 4 / 8 150 / 150 / 156.
+    # Rows of few tiles and launches of many blocks are not cut: putting runs together is another launch. us of 12 blocks of 16 tiles in 1 / 4 / 8 runs 7.5 / 8.2 /
+    # 8.1; of 200 of 15 (32-bit) in 1 / 3 / 5 11.1 / 14.3 / 13.6; of 768 of 63 in 1 / 3 / 5 68 / 73 / 65. Others are cut until there are two blocks for each of
+    # 256 compute units, into at most about sqrt(tiles) runs: of 12 of 63 in 3 / 5 / 9 / 21 11.4 / 10.5 / 9.4 / 9.6; of 8 of 469 (heads of 128) in 5 / 9 / 17 / 34 / 59
+    # 33 / 25 / 23 / 31 / 30; of 96 of 63 (32-bit) in 1 / 5 / 9 / 21 22.2 / 18.6 / 19.4 / 19.4; of 128 of 480 in 1 / 2 / 4 / 8 212 / 167 / 149 / 157.
     runs = 1 if tiles <= 2 * most else max(1, min(512 // max(blocks, 1), round(0.8 * tiles**0.5)))
     run = -(-tiles // runs)
     runs = -(-tiles // run)
-    # Waves: as many as have a tile, up to 12 a compute unit (768 blocks of 16 tiles with 2 / 4 / 8 waves 15.5 / 15.3 / 17.3; 512 14.3 / 12.4 / 13.0).
+    # Waves: as many as have a tile, up to 12 a compute unit (768 blocks of 16 tiles with 2 / 4 / 8 waves 16.1 / 15.6 / 17.2; 512 15.2 / 12.1 / 12.6).
     waves = 1
     while waves < most and waves < run and 2 * waves * blocks * runs <= 12 * 256:
         waves *= 2
@@ -1673,9 +1673,9 @@ def scaled_cut(blocks: int, tiles: int, head_size: int, columns: int, wide: bool
 def scaled_mixes(row_blocks: int, rows: int, requests: int, longest: int, n_heads: int, head_size: int, wide: bool = False) -> bool:
     """Whether a step's decoding rows (``row_blocks`` (row, head group) pairs) and its portions (``rows`` of ``requests``, up to ``longest`` each) go in one launch over
     pages of 8 bits. There the portions' blocks have half the rows that they may have by themselves, and rows four waves."""
-    # us in one / two launches (and a merge where rows are cut), 12 heads of 64 in bfloat16, rows at 900 keys beside a portion of 512: 1 row 7.1 / 13.0, 8 8.3 / 15.1, 32 15.5 / 18.9,
-    # 64 23.0 / 26.5, 128 (1,536 pairs) 43.4 / 46.3, 256 77.7 / 77.1; 32 rows beside 2,048 (384 blocks of whole tiles) 26.6 / 31.3, 20 heads (640) 40.1 / 45.1, 25 (800) 52.7 / 54.1, with 64 rows
-    # 71.4 / 70.6; 32 heads of 128 on 8, 16 rows at 2,000 beside 512 (512 blocks) 31.9 / 31.1, 32 beside 1,024 (1,024) 63.6 / 58.6, 2,048 (2,048) 113 / 86; in 32-bit (whose tiles are as
+    # us in one / two launches (and a merge where rows are cut), 12 heads of 64 in bfloat16, rows at 900 keys beside a portion of 512: 1 row 7.4 / 13.5, 8 8.9 / 15.5, 32 15.7 / 19.5,
+    # 64 23.6 / 26.8, 128 (1,536 pairs) 44.0 / 46.8, 256 78.8 / 77.4; 32 rows beside 2,048 (384 blocks of whole tiles) 26.8 / 31.6, 20 heads (640) 40.1 / 45.3, 25 (800) 53.7 / 55.7, with 64 rows
+    # 73.6 / 73.4; 32 heads of 128 on 8, 16 rows at 2,000 beside 512 (512 blocks) 32.0 / 31.2, 32 beside 1,024 (1,024) 63.9 / 58.9, 2,048 (2,048) 113 / 85; in 32-bit (whose tiles are as
     # large in either, or lose less) 64 rows beside 512 24.4 / 29.4, 25 heads, 32 rows beside 2,016 (1,600) 79.8 / 90.5, 32 heads of 128 beside 1,024 (1,024) 76.6 / 82.8.
     tile, most = (32, 2048) if wide else (64, 832) if head_size <= 64 else (32, 512)
     return head_size <= 128 and row_blocks <= 2048 and n_heads * min(rows // tile + requests, requests * -(-longest // tile)) <= most
